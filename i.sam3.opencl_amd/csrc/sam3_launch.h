@@ -343,6 +343,82 @@ int launch_dec_heads(const float *qry, const void *const w0[4],
 int launch_convert(const float *src, void *dst, int dst_dt, size_t count,
                    void *stream);
 
+/* ------------------------------------------------ cross attention */
+
+/* cross_attend: heads = grp x kvh, unit = batch x kv head; the offsets and
+ * strides of struct opnd per operand. The fields after `c` are set by
+ * xattn_ws / launch_xattn. */
+struct xattn_desc {
+    const void *Q, *K, *V;
+    void *O;
+    long qo, qs0, qs1, ko, ks0, ks1, vo, vs0, vs1, oo, os0, os1;
+    int qld, kld, vld, old;
+    int qvec, kvec, vvec, ovec; /* 16-byte accesses of whole rows fit */
+    const int *qlen, *klen;
+    const unsigned char *kmask;
+    int units, kvh, grp, hd, Nq, Nk, dt;
+    float c; /* scale log2 e */
+    int wm, tiles, splits, heads_first, pvec;
+    long items;
+    float *part; /* [split][unit][grp Nq] rows of hd sums, then (m, sum) */
+    long part_ml;
+};
+
+/* Bytes of workspace that lets launch_xattn split the keys (0: it does not
+ * want to); with less, or NULL, one workgroup walks all keys of its rows. */
+size_t xattn_ws(struct xattn_desc *d);
+int launch_xattn(struct xattn_desc *d, void *ws, size_t ws_bytes, void *stream);
+
+/* ------------------------------------------------ rotary positions */
+
+#define ROPE_MAX_PAIRS 256
+
+/* Table rows (cos, sin) of npos positions (pos[p], or p): angle of pair j =
+ * turns[j] x (position, or its column j < pairs / 2 and row in a grid W wide)
+ * in turns, times mul. */
+struct rope_table_desc {
+    float *table;
+    const int *pos;
+    int npos, pairs, W;
+    float mul;
+    double turns[ROPE_MAX_PAIRS];
+};
+int launch_rope_table(const struct rope_table_desc *d, void *stream);
+
+/* rope_rows: rows of nb batches x heads; position pos[b rows + r], or (pos0 +
+ * r) % npos. vec: 16-byte accesses fit; copy: Y is not X. */
+struct rope_rows_desc {
+    const void *X;
+    void *Y;
+    long xo, xs0, xs1, yo, ys0, ys1;
+    int xld, yld;
+    int nb, heads, rows, hd, rot, halves, npos, dt, vec, copy;
+    const float *table;
+    const int *pos;
+    long pos0;
+};
+int launch_rope_rows(const struct rope_rows_desc *d, void *stream);
+
+/* ------------------------------------------------ group norm */
+
+struct groupnorm_desc {
+    const void *X;
+    void *Y;
+    long xo, xs0, yo, ys0;
+    int xld, yld;
+    int nb, C, groups, dt, act, vec;
+    long rows;
+    const float *g, *b;
+    float eps;
+    int chunks; /* set by groupnorm_ws_bytes / launch_groupnorm */
+    float *part;
+};
+
+/* Workspace (0: none wanted); with less, or NULL, one workgroup per (batch,
+ * group) walks all rows. */
+size_t groupnorm_ws_bytes(struct groupnorm_desc *d);
+int launch_groupnorm(struct groupnorm_desc *d, void *ws, size_t ws_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1580,3 +1580,514 @@ void sam_path_free(struct sam_model *m)
     hipb_release(&m->askrec);
     hipb_release(&m->askcnt);
 }
+
+/* ------------------------------------------------------------ other sequences */
+
+/* Largest row stride that the kernels' 32-bit row offsets inside a tile
+ * reach, in bytes. */
+#define ROW_STRIDE_MAX (16L << 20)
+/* Threads of a launch's x dimension. */
+#define GRID_MAX 0xffffffffL
+
+static long elem_size(int dtype)
+{
+    return dtype == HIPB_F32 ? 4 : 2;
+}
+
+/* First and last element of nb batches x heads of rows x cols of o. */
+static void opnd_span(struct opnd o, int nb, int heads, long rows, long cols, long *first,
+                      long *last)
+{
+    *first = o.off;
+    *last = o.off + (nb - 1) * o.s0 + (heads - 1) * o.s1 + (rows - 1) * (long)o.ld + cols - 1;
+}
+
+/* Do two operands (spans as above) share memory? */
+static int spans_meet(struct opnd a, const long *sa, struct opnd b, const long *sb)
+{
+    const long za = elem_size(a.buf->dtype), zb = elem_size(b.buf->dtype);
+    const char *pa = a.buf->ptr, *pb = b.buf->ptr;
+
+    return pa + sa[0] * za < pb + (sb[1] + 1) * zb && pb + sb[0] * zb < pa + (sa[1] + 1) * za;
+}
+
+/* True if no two elements of an output operand (nb x heads x rows x cols) are
+ * the same: its dimensions in order of their strides, each past the end of
+ * those below it. */
+static int opnd_distinct(const char *op, const char *name, struct opnd o, int nb, int heads,
+                         long rows, long cols)
+{
+    long st[3] = {o.s0, o.s1, o.ld}, n[3] = {nb, heads, rows}, end = cols;
+    int i, j;
+
+    for (i = 0; i < 3; i++)
+        for (j = i + 1; j < 3; j++)
+            if (st[j] < st[i]) {
+                long t = st[i];
+
+                st[i] = st[j];
+                st[j] = t;
+                t = n[i];
+                n[i] = n[j];
+                n[j] = t;
+            }
+    for (i = 0; i < 3; i++) {
+        if (n[i] == 1)
+            continue;
+        if (st[i] < end) {
+            hipb_fatal("%s: output operand %s writes elements twice (strides %ld %ld %d)", op,
+                       name, o.s0, o.s1, o.ld);
+            return 0;
+        }
+        end += (n[i] - 1) * st[i];
+    }
+    return 1;
+}
+
+/* True if every row of the operand starts on 16 bytes. */
+static int opnd_vec(struct opnd o, int nb, int heads, long rows)
+{
+    const long v = 16 / elem_size(o.buf->dtype);
+
+    return (uintptr_t)o.buf->ptr % 16 == 0 && o.off % v == 0 && (nb == 1 || o.s0 % v == 0) &&
+           (heads == 1 || o.s1 % v == 0) && (rows == 1 || o.ld % v == 0);
+}
+
+/* A plain buffer of n bytes (integers, masks). */
+static int bytes_ok(const char *op, const char *name, hipb_mem m, size_t n)
+{
+    if (m && m->bytes >= n && (uintptr_t)m->ptr % 4 == 0)
+        return 1;
+    hipb_fatal("%s: %s <%s> holds %lu bytes, %lu needed", op, name, m ? m->what : "none",
+               m ? (unsigned long)m->bytes : 0ul, (unsigned long)n);
+    return 0;
+}
+
+/* The caller's workspace, checked, or the backend's (NULL where that cannot
+ * be had: the kernels then do without). 0 on error. */
+static int workspace(struct hipb_backend *b, const char *op, hipb_mem ws, size_t need, void **p,
+                     size_t *bytes)
+{
+    *p = NULL;
+    *bytes = 0;
+    if (ws) {
+        if (ws->bytes < need || (uintptr_t)ws->ptr % 16) {
+            hipb_fatal("%s: workspace <%s> holds %lu bytes, %lu needed (16-byte aligned)", op,
+                       ws->what, (unsigned long)ws->bytes, (unsigned long)need);
+            return 0;
+        }
+        *p = ws->ptr;
+        *bytes = ws->bytes;
+    }
+    else if (need) {
+        *p = hipb_gemm_ws(b, need);
+        *bytes = *p ? need : 0;
+    }
+    return 1;
+}
+
+/* Makes the backend's device the thread's current one; returns the one to
+ * go back to. */
+static int device_enter(const struct hipb_backend *b)
+{
+    int old = b->device;
+
+    if (hipGetDevice(&old) == hipSuccess && old != b->device)
+        (void)hipSetDevice(b->device);
+    return old;
+}
+
+static void device_leave(const struct hipb_backend *b, int old)
+{
+    if (old != b->device)
+        (void)hipSetDevice(old);
+}
+
+/* Shape of cross_attend as its kernels take it; 0 on error. */
+static int xattn_shape(struct xattn_desc *d, const char *op, int nb, int heads, int kv_heads,
+                       int hd, int Nq, int Nk, int dtype)
+{
+    if (nb < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads || hd < 1 || hd > 256 || Nq < 0 ||
+        Nk < 0) {
+        hipb_fatal("%s: invalid shape nb=%d heads=%d kv_heads=%d hd=%d Nq=%d Nk=%d (kv_heads "
+                   "divides heads, hd is at most 256)",
+                   op, nb, heads, kv_heads, hd, Nq, Nk);
+        return 0;
+    }
+    if (dtype != HIPB_F32 && dtype != HIPB_F16 && dtype != HIPB_BF16) {
+        hipb_fatal("%s: unknown element type %d", op, dtype);
+        return 0;
+    }
+    /* Rows and work items are counted in 32 bits. */
+    if ((long)nb * heads > 1L << 22 || (long)heads / kv_heads * Nq > 0x7fffffffL - 128 ||
+        (double)nb * heads * Nq > 6.4e7) {
+        hipb_fatal("%s: too many rows (nb=%d heads=%d Nq=%d)", op, nb, heads, Nq);
+        return 0;
+    }
+    memset(d, 0, sizeof(*d));
+    d->units = nb * kv_heads;
+    d->kvh = kv_heads;
+    d->grp = heads / kv_heads;
+    d->hd = hd;
+    d->Nq = Nq;
+    d->Nk = Nk;
+    d->dt = dtype;
+    return 1;
+}
+
+size_t cross_attend_ws(struct sam_model *m, int nb, int heads, int kv_heads, int hd, int Nq,
+                       int Nk, int dtype)
+{
+    struct xattn_desc d;
+
+    if (!xattn_shape(&d, "cross_attend_ws", nb, heads, kv_heads, hd, Nq, Nk, dtype) || nb == 0 ||
+        Nq == 0)
+        return 0;
+    return xattn_ws(&d);
+}
+
+void cross_attend(struct sam_model *m, int nb, int heads, int kv_heads, int hd, int Nq, int Nk,
+                  struct opnd Q, struct opnd K, struct opnd V, struct opnd O, hipb_mem qlen,
+                  hipb_mem klen, hipb_mem kmask, float scale, hipb_mem ws)
+{
+    static const char op[] = "cross_attend";
+    struct hipb_backend *be = m->hip;
+    struct xattn_desc d;
+    long so[2], si[2];
+    const struct opnd *in[3] = {&Q, &K, &V};
+    size_t ws_bytes, need;
+    void *wp;
+    int err, old, i;
+
+    if (!Q.buf || !K.buf || !V.buf || !O.buf) {
+        hipb_fatal("%s: operand without a buffer", op);
+        return;
+    }
+    if (!xattn_shape(&d, op, nb, heads, kv_heads, hd, Nq, Nk, Q.buf->dtype))
+        return;
+    if (K.buf->dtype != d.dt || V.buf->dtype != d.dt || O.buf->dtype != d.dt) {
+        hipb_fatal("%s: Q, K, V and O have one element type (%d %d %d %d)", op, Q.buf->dtype,
+                   K.buf->dtype, V.buf->dtype, O.buf->dtype);
+        return;
+    }
+    if (!(scale > 0.0f) || isinf(scale)) {
+        hipb_fatal("%s: scale %g is not positive and finite", op, (double)scale);
+        return;
+    }
+    if (nb == 0 || Nq == 0)
+        return;
+    if (!opnd_ok(op, "Q", Q, Nq, hd, nb * heads, heads) ||
+        !opnd_ok(op, "K", K, Nk, hd, nb * kv_heads, kv_heads) ||
+        !opnd_ok(op, "V", V, Nk, hd, nb * kv_heads, kv_heads) ||
+        !opnd_ok(op, "O", O, Nq, hd, nb * heads, heads) ||
+        !opnd_distinct(op, "O", O, nb, heads, Nq, hd))
+        return;
+    if (K.ld * elem_size(d.dt) > ROW_STRIDE_MAX || V.ld * elem_size(d.dt) > ROW_STRIDE_MAX) {
+        hipb_fatal("%s: rows of K or V are more than 16 MiB apart", op);
+        return;
+    }
+    opnd_span(O, nb, heads, Nq, hd, &so[0], &so[1]);
+    for (i = 0; i < 3; i++) {
+        if (i && Nk == 0)
+            break;
+        opnd_span(*in[i], nb, i ? kv_heads : heads, i ? Nk : Nq, hd, &si[0], &si[1]);
+        if (spans_meet(O, so, *in[i], si)) {
+            hipb_fatal("%s: O overlaps %c", op, "QKV"[i]);
+            return;
+        }
+    }
+    if ((qlen && !bytes_ok(op, "qlen", qlen, 4 * (size_t)nb)) ||
+        (klen && !bytes_ok(op, "klen", klen, 4 * (size_t)nb)) ||
+        (kmask && !bytes_ok(op, "kmask", kmask, (size_t)nb * Nk)))
+        return;
+    need = xattn_ws(&d);
+    if (!workspace(be, op, ws, need, &wp, &ws_bytes))
+        return;
+    d.Q = Q.buf->ptr;
+    d.qo = Q.off;
+    d.qs0 = Q.s0;
+    d.qs1 = Q.s1;
+    d.qld = Q.ld;
+    d.K = K.buf->ptr;
+    d.ko = K.off;
+    d.ks0 = K.s0;
+    d.ks1 = K.s1;
+    d.kld = K.ld;
+    d.V = V.buf->ptr;
+    d.vo = V.off;
+    d.vs0 = V.s0;
+    d.vs1 = V.s1;
+    d.vld = V.ld;
+    d.O = O.buf->ptr;
+    d.oo = O.off;
+    d.os0 = O.s0;
+    d.os1 = O.s1;
+    d.old = O.ld;
+    i = hd * elem_size(d.dt) % 16 == 0;
+    d.qvec = i && opnd_vec(Q, nb, heads, Nq);
+    d.kvec = i && opnd_vec(K, nb, kv_heads, Nk);
+    d.vvec = i && opnd_vec(V, nb, kv_heads, Nk);
+    d.ovec = i && opnd_vec(O, nb, heads, Nq);
+    d.pvec = hd % 4 == 0;
+    d.qlen = qlen ? qlen->ptr : NULL;
+    d.klen = klen ? klen->ptr : NULL;
+    d.kmask = kmask ? kmask->ptr : NULL;
+    d.c = scale * LOG2E_HOST;
+    old = device_enter(be);
+    hipb_run_begin(be);
+    err = launch_xattn(&d, wp, ws_bytes, be->stream);
+    hipb_run_end(be, err, op, 4.0 * nb * heads * (double)Nq * Nk * hd);
+    device_leave(be, old);
+}
+
+void rope_table(struct sam_model *m, hipb_mem table, int npos, hipb_mem pos, int rot, int W,
+                double theta, const struct rope_scale *sc)
+{
+    static const char op[] = "rope_table";
+    struct hipb_backend *be = m->hip;
+    const int kind = sc ? sc->kind : ROPE_PLAIN;
+    const double s = kind != ROPE_PLAIN ? sc->factor : 1.0;
+    const double two_pi = 6.283185307179586476925;
+    struct rope_table_desc d;
+    int err, old, j;
+
+    if (npos < 0 || rot < 2 || rot % 2 || rot > 2 * ROPE_MAX_PAIRS || W < 0 || (W && rot % 4) ||
+        !(theta > 0.0) || isinf(theta)) {
+        hipb_fatal("%s: invalid npos=%d rot=%d W=%d theta=%g (rot is even, at most %d, and a "
+                   "multiple of 4 over a grid)",
+                   op, npos, rot, W, theta, 2 * ROPE_MAX_PAIRS);
+        return;
+    }
+    if (kind < ROPE_PLAIN || kind > ROPE_YARN || !(s >= 1.0) || isinf(s) ||
+        (kind != ROPE_PLAIN && W) || (kind == ROPE_NTK && rot < 4) ||
+        (kind == ROPE_YARN && (sc->orig < 1 || !(sc->beta_slow >= 0.0) ||
+                               !(sc->beta_fast > sc->beta_slow) || isinf(sc->beta_fast)))) {
+        hipb_fatal("%s: invalid scaling (kind %d, factor %g)", op, kind, s);
+        return;
+    }
+    if (!buf_ok(op, "table", table, (size_t)npos * rot, HIPB_F32) ||
+        (pos && !bytes_ok(op, "pos", pos, 4 * (size_t)npos)))
+        return;
+    if ((uintptr_t)table->ptr % 8) {
+        hipb_fatal("%s: table is not 8-byte aligned", op);
+        return;
+    }
+    if ((long)npos * (rot / 2) > GRID_MAX - 256) {
+        hipb_fatal("%s: more than 2^32 angles", op);
+        return;
+    }
+    if (npos == 0)
+        return;
+    d.table = table->ptr;
+    d.pos = pos ? pos->ptr : NULL;
+    d.npos = npos;
+    d.pairs = rot / 2;
+    d.W = W;
+    d.mul = kind == ROPE_YARN ? (float)(0.1 * log(s) + 1.0) : 1.0f;
+    if (kind == ROPE_NTK)
+        theta *= pow(s, rot / (rot - 2.0));
+    for (j = 0; j < d.pairs; j++) {
+        double f = W ? pow(theta, -4.0 * (j % (rot / 4)) / rot) : pow(theta, -2.0 * j / rot);
+
+        if (kind == ROPE_LINEAR)
+            f /= s;
+        else if (kind == ROPE_YARN) {
+            /* Turns that the pair makes within the original context: many
+             * (beta_fast) and it stays, few (beta_slow) and it is stretched. */
+            double g = (sc->orig * f / two_pi - sc->beta_slow) / (sc->beta_fast - sc->beta_slow);
+
+            g = g < 0.0 ? 0.0 : g > 1.0 ? 1.0 : g;
+            f = (1.0 - g) * f / s + g * f;
+        }
+        d.turns[j] = f / two_pi;
+    }
+    old = device_enter(be);
+    hipb_run_begin(be);
+    err = launch_rope_table(&d, be->stream);
+    hipb_run_end(be, err, op, 0.0);
+    device_leave(be, old);
+}
+
+void rope_rows(struct sam_model *m, int nb, int heads, int rows, int hd, int rot, int layout,
+               struct opnd X, struct opnd Y, hipb_mem table, int npos, hipb_mem pos, long pos0)
+{
+    static const char op[] = "rope_rows";
+    struct hipb_backend *be = m->hip;
+    struct rope_rows_desc d;
+    long sx[2], sy[2];
+    int err, old, v, same;
+
+    if (nb < 0 || heads < 1 || rows < 0 || hd < 2 || rot < 2 || rot % 2 || rot > hd || npos < 1 ||
+        pos0 < 0 || pos0 > 0x7fffffffL || (layout != ROPE_PAIRS && layout != ROPE_HALVES)) {
+        hipb_fatal("%s: invalid shape nb=%d heads=%d rows=%d hd=%d rot=%d layout=%d npos=%d "
+                   "pos0=%ld",
+                   op, nb, heads, rows, hd, rot, layout, npos, pos0);
+        return;
+    }
+    if (nb == 0 || rows == 0)
+        return;
+    if ((long)nb * heads > 0x7fffffffL) {
+        hipb_fatal("%s: too many heads (nb=%d heads=%d)", op, nb, heads);
+        return;
+    }
+    if (!opnd_ok(op, "X", X, rows, hd, nb * heads, heads) ||
+        !opnd_ok(op, "Y", Y, rows, hd, nb * heads, heads) ||
+        !opnd_distinct(op, "Y", Y, nb, heads, rows, hd) ||
+        !buf_ok(op, "table", table, (size_t)npos * rot, HIPB_F32) ||
+        (pos && !bytes_ok(op, "pos", pos, 4 * (size_t)nb * rows)))
+        return;
+    if (X.buf->dtype != Y.buf->dtype || (uintptr_t)table->ptr % 8) {
+        hipb_fatal("%s: X and Y have one element type, the table is 8-byte aligned", op);
+        return;
+    }
+    /* In place, or apart. */
+    same = (char *)X.buf->ptr + X.off * elem_size(X.buf->dtype) ==
+               (char *)Y.buf->ptr + Y.off * elem_size(Y.buf->dtype) &&
+           (rows == 1 || X.ld == Y.ld) && (nb == 1 || X.s0 == Y.s0) &&
+           (heads == 1 || X.s1 == Y.s1);
+    opnd_span(X, nb, heads, rows, hd, &sx[0], &sx[1]);
+    opnd_span(Y, nb, heads, rows, hd, &sy[0], &sy[1]);
+    if (!same && spans_meet(X, sx, Y, sy)) {
+        hipb_fatal("%s: Y overlaps X and is not X", op);
+        return;
+    }
+    if ((double)nb * rows * hd > 4e9) {
+        hipb_fatal("%s: too many rows (nb=%d rows=%d)", op, nb, rows);
+        return;
+    }
+    memset(&d, 0, sizeof(d));
+    d.X = X.buf->ptr;
+    d.xo = X.off;
+    d.xs0 = X.s0;
+    d.xs1 = X.s1;
+    d.xld = X.ld;
+    d.Y = Y.buf->ptr;
+    d.yo = Y.off;
+    d.ys0 = Y.s0;
+    d.ys1 = Y.s1;
+    d.yld = Y.ld;
+    d.nb = nb;
+    d.heads = heads;
+    d.rows = rows;
+    d.hd = hd;
+    d.rot = rot;
+    d.halves = layout == ROPE_HALVES;
+    d.npos = npos;
+    d.dt = X.buf->dtype;
+    v = 16 / (int)elem_size(d.dt);
+    d.vec = opnd_vec(X, nb, heads, rows) && opnd_vec(Y, nb, heads, rows) &&
+            (d.halves ? rot / 2 : rot) % v == 0 && (hd - rot) % v == 0;
+    d.copy = !same;
+    d.table = table->ptr;
+    d.pos = pos ? pos->ptr : NULL;
+    d.pos0 = pos0;
+    old = device_enter(be);
+    hipb_run_begin(be);
+    err = launch_rope_rows(&d, be->stream);
+    hipb_run_end(be, err, op, 0.0);
+    device_leave(be, old);
+}
+
+/* Shape of groupnorm; 0 on error. */
+static int gn_shape(struct groupnorm_desc *d, const char *op, int nb, long rows, int C, int groups,
+                    int dtype)
+{
+    if (nb < 0 || nb > 65535 || rows < 0 || C < 1 || groups < 1 || groups > 4096 || C % groups) {
+        hipb_fatal("%s: invalid shape nb=%d rows=%ld C=%d groups=%d (groups divide C, at most "
+                   "4096)",
+                   op, nb, rows, C, groups);
+        return 0;
+    }
+    if (dtype != HIPB_F32 && dtype != HIPB_F16 && dtype != HIPB_BF16) {
+        hipb_fatal("%s: unknown element type %d", op, dtype);
+        return 0;
+    }
+    memset(d, 0, sizeof(*d));
+    d->nb = nb;
+    d->rows = rows;
+    d->C = C;
+    d->groups = groups;
+    d->dt = dtype;
+    return 1;
+}
+
+size_t groupnorm_ws(struct sam_model *m, int nb, long rows, int C, int groups, int dtype)
+{
+    struct groupnorm_desc d;
+
+    if (!gn_shape(&d, "groupnorm_ws", nb, rows, C, groups, dtype) || nb == 0 || rows == 0)
+        return 0;
+    return groupnorm_ws_bytes(&d);
+}
+
+void groupnorm(struct sam_model *m, int nb, long rows, int C, int groups, struct opnd X,
+               struct opnd Y, hipb_mem g, hipb_mem b, float eps, int act, hipb_mem ws)
+{
+    static const char op[] = "groupnorm";
+    struct hipb_backend *be = m->hip;
+    struct groupnorm_desc d;
+    long sx[2], sy[2], v;
+    size_t ws_bytes, need;
+    void *wp;
+    int err, old, same;
+
+    if (!X.buf || !Y.buf) {
+        hipb_fatal("%s: operand without a buffer", op);
+        return;
+    }
+    if (!gn_shape(&d, op, nb, rows, C, groups, X.buf->dtype))
+        return;
+    if (act < ACT_NONE || act > ACT_SILU || !(eps >= 0.0f) || isinf(eps)) {
+        hipb_fatal("%s: invalid act=%d eps=%g", op, act, (double)eps);
+        return;
+    }
+    if (Y.buf->dtype != d.dt) {
+        hipb_fatal("%s: X and Y have one element type", op);
+        return;
+    }
+    if (nb == 0 || rows == 0)
+        return;
+    X.s1 = Y.s1 = 0;
+    if (!opnd_ok(op, "X", X, rows, C, nb, 1) || !opnd_ok(op, "Y", Y, rows, C, nb, 1) ||
+        !opnd_distinct(op, "Y", Y, nb, 1, rows, C) ||
+        (g && !buf_ok(op, "g", g, (size_t)C, HIPB_F32)) ||
+        (b && !buf_ok(op, "b", b, (size_t)C, HIPB_F32)))
+        return;
+    same = (char *)X.buf->ptr + X.off * elem_size(d.dt) ==
+               (char *)Y.buf->ptr + Y.off * elem_size(d.dt) &&
+           (rows == 1 || X.ld == Y.ld) && (nb == 1 || X.s0 == Y.s0);
+    opnd_span(X, nb, 1, rows, C, &sx[0], &sx[1]);
+    opnd_span(Y, nb, 1, rows, C, &sy[0], &sy[1]);
+    if (!same && spans_meet(X, sx, Y, sy)) {
+        hipb_fatal("%s: Y overlaps X and is not X", op);
+        return;
+    }
+    need = groupnorm_ws_bytes(&d);
+    if (!workspace(be, op, ws, need, &wp, &ws_bytes))
+        return;
+    d.X = X.buf->ptr;
+    d.xo = X.off;
+    d.xs0 = X.s0;
+    d.xld = X.ld;
+    d.Y = Y.buf->ptr;
+    d.yo = Y.off;
+    d.ys0 = Y.s0;
+    d.yld = Y.ld;
+    d.g = g ? g->ptr : NULL;
+    d.b = b ? b->ptr : NULL;
+    d.eps = eps;
+    d.act = act;
+    /* Elements taken together: they lie in one group and are aligned. */
+    for (v = 16 / elem_size(d.dt); v > 1; v /= 2)
+        if (C / groups % v == 0 && X.off % v == 0 && Y.off % v == 0 &&
+            (nb == 1 || (X.s0 % v == 0 && Y.s0 % v == 0)) &&
+            (rows == 1 || (X.ld % v == 0 && Y.ld % v == 0)) &&
+            ((uintptr_t)X.buf->ptr | (uintptr_t)Y.buf->ptr) % (v * elem_size(d.dt)) == 0)
+            break;
+    d.vec = (int)v;
+    old = device_enter(be);
+    hipb_run_begin(be);
+    err = launch_groupnorm(&d, wp, ws_bytes, be->stream);
+    hipb_run_end(be, err, op, 0.0);
+    device_leave(be, old);
+}

@@ -19,7 +19,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "libsam3hip.so")
 
 F32, F16, BF16 = 0, 1, 2
-ACT_NONE, ACT_GELU, ACT_RELU = 0, 1, 2
+ACT_NONE, ACT_GELU, ACT_RELU, ACT_SILU = 0, 1, 2, 3
+ROPE_PAIRS, ROPE_HALVES = 0, 1
+ROPE_PLAIN, ROPE_LINEAR, ROPE_NTK, ROPE_YARN = 0, 1, 2, 3
 ERR_FATAL, ERR_RECORD = 0, 1
 
 # Every symbol include/sam3_hip.h declares.
@@ -40,7 +42,8 @@ EXPORTS = [
     "i2t_attention", "convt_scatter", "sam_postprocess", "sam_read_mask",
     "sam_dec_graph", "mask_logits", "pth_upload", "load_dev", "load_dev_w",
     "load_dev_fmt", "load_dev_w_fmt", "load_host", "load_host_into",
-    "sam_load", "sam_free", "sam_is_sam3",
+    "sam_load", "sam_free", "sam_is_sam3", "cross_attend", "cross_attend_ws",
+    "rope_table", "rope_rows", "groupnorm", "groupnorm_ws",
 ]
 # include/pth_loader.h
 PTH_EXPORTS = [
@@ -84,6 +87,12 @@ class HipbBackend(ctypes.Structure):
 class Opnd(ctypes.Structure):
     _fields_ = [("buf", Mem), ("off", ctypes.c_long), ("ld", ctypes.c_int),
                 ("s0", ctypes.c_long), ("s1", ctypes.c_long)]
+
+
+class RopeScale(ctypes.Structure):
+    _fields_ = [("kind", ctypes.c_int), ("factor", ctypes.c_double),
+                ("orig", ctypes.c_int), ("beta_fast", ctypes.c_double),
+                ("beta_slow", ctypes.c_double)]
 
 
 class VitBlock(ctypes.Structure):
@@ -274,6 +283,18 @@ def lib():
                                   vp]
     L.sam_read_mask.argtypes = [MP, c_int, c_int, c_int, c_int, c_int, c_int,
                                 c_int, vp]
+    L.cross_attend.argtypes = [MP] + [c_int] * 6 + [Opnd] * 4 + [Mem] * 3 + \
+        [c_float, Mem]
+    L.cross_attend_ws.argtypes = [MP] + [c_int] * 7
+    L.cross_attend_ws.restype = c_size
+    L.rope_table.argtypes = [MP, Mem, c_int, Mem, c_int, c_int,
+                             ctypes.c_double, ctypes.POINTER(RopeScale)]
+    L.rope_rows.argtypes = [MP] + [c_int] * 6 + [Opnd, Opnd, Mem, c_int, Mem,
+                                                c_long]
+    L.groupnorm.argtypes = [MP, c_int, c_long, c_int, c_int, Opnd, Opnd, Mem,
+                            Mem, c_float, c_int, Mem]
+    L.groupnorm_ws.argtypes = [MP, c_int, c_long, c_int, c_int, c_int]
+    L.groupnorm_ws.restype = c_size
     FP = ctypes.POINTER(PthFile)
     TP = ctypes.POINTER(PthTensor)
     LP = ctypes.POINTER(c_long)
@@ -593,6 +614,13 @@ def bmat(buf, off, ld, s0, s1):
     return Opnd(buf, off, ld, s0, s1)
 
 
+def borrow(ptr, nbytes, dtype=F32, what="borrowed"):
+    """A handle of device memory that another allocator owns (struct hipb_buf
+    is plain data): for the operators, never for hipb_release. The memory has
+    to outlive the handle's calls."""
+    return ctypes.pointer(HipbBuf(ptr, nbytes, dtype, what.encode()))
+
+
 def _call(fn, *args):
     fn(*args)
     _check()
@@ -681,6 +709,42 @@ def sam_trunk_graph(m, enable=True):
     """Capture the trunk's kernels into a HIP graph that later
     sam_encode_trunk calls replay (enable=False drops it)."""
     _call(_lib.sam_trunk_graph, m.ptr, int(bool(enable)))
+
+
+def cross_attend(m, nb, heads, kv_heads, hd, Nq, Nk, Q, K, V, O, qlen=None,
+                 klen=None, kmask=None, scale=None, ws=None):
+    """scale: 1 / sqrt(hd) unless given."""
+    _call(_lib.cross_attend, m.ptr, nb, heads, kv_heads, hd, Nq, Nk, Q, K, V, O,
+          qlen, klen, kmask, max(hd, 1) ** -0.5 if scale is None else scale, ws)
+
+
+def cross_attend_ws(m, nb, heads, kv_heads, hd, Nq, Nk, dtype):
+    n = _lib.cross_attend_ws(m.ptr, nb, heads, kv_heads, hd, Nq, Nk, dtype)
+    _check()
+    return n
+
+
+def rope_table(m, table, npos, pos=None, rot=64, W=0, theta=10000.0, scale=None):
+    """scale: a RopeScale, or None."""
+    _call(_lib.rope_table, m.ptr, table, npos, pos, rot, W, theta,
+          None if scale is None else ctypes.byref(scale))
+
+
+def rope_rows(m, nb, heads, rows, hd, rot, layout, X, Y, table, npos, pos=None,
+              pos0=0):
+    _call(_lib.rope_rows, m.ptr, nb, heads, rows, hd, rot, layout, X, Y, table,
+          npos, pos, pos0)
+
+
+def groupnorm(m, nb, rows, C, groups, X, Y, g=None, b=None, eps=1e-5,
+              act=ACT_NONE, ws=None):
+    _call(_lib.groupnorm, m.ptr, nb, rows, C, groups, X, Y, g, b, eps, act, ws)
+
+
+def groupnorm_ws(m, nb, rows, C, groups, dtype):
+    n = _lib.groupnorm_ws(m.ptr, nb, rows, C, groups, dtype)
+    _check()
+    return n
 
 
 def prof_table():

@@ -398,6 +398,101 @@ void sam_encode_trunk(struct sam_model *m, const float *img);
 void sam_trunk_graph(struct sam_model *m, int enable);
 
 /* ------------------------------------------------------------------ */
+/* Attention to another sequence, rotary positions, group norm         */
+/* ------------------------------------------------------------------ */
+
+/* Of these operators the reference has groupnorm_relu (sam3_kernels.cl:
+ * 923-953); the others serve models that attend to prompts, earlier frames or
+ * an encoder's states. Operands are f32, f16 or bf16, whatever the backend's
+ * precision, and are computed as such: products of floats are float products,
+ * those of halves and bf16 are exact; sums, maxima and statistics are f32
+ * or wider, results are rounded once. (P of half and bf16 attention is rounded
+ * to the operands' type, as the product with V takes it.) Integers, positions
+ * and masks lie in plain buffers (hipb_alloc). The operators queue kernels
+ * only and may be captured; see `ws` for their workspace. */
+
+/* Cross attention: for batch b < nb, head h < heads and query i < qlen[b]
+ * (Nq where qlen is NULL),
+ *   O[b][i][h] = sum_j softmax_j(scale Q[b][i][h] . K[b][j][g]) V[b][j][g]
+ * over the keys j < klen[b] (Nk) with kmask[b][j] != 0 (all), g = h / (heads /
+ * kv_heads). Row i of batch b and head h lies at off + b s0 + h s1 + i ld of
+ * its operand, hd <= 256 columns; any such layout is taken, whole rows on 16
+ * bytes fastest. Q, K, V and O have one element type, O overlaps none of the
+ * others. qlen, klen: nb int32 (clamped to 0 .. Nq, Nk); kmask: [nb][Nk]
+ * bytes. What stands in masked keys and values, or behind the lengths, is
+ * not used, NaN or infinity neither; a query without a key, or whose scores
+ * are all minus infinity, gives zeros; rows of O behind qlen are left as they
+ * are. scale is positive.
+ * Few rows over many keys are split over workgroups, whose partial sums go to
+ * ws: at least cross_attend_ws bytes of the caller's, which calls that may
+ * overlap (other streams, graphs) must not share; or NULL for the backend's
+ * own workspace, which a call that the caller captures does without (one
+ * workgroup then walks all keys of its rows; results differ by rounding). */
+void cross_attend(struct sam_model *m, int nb, int heads, int kv_heads, int hd,
+                  int Nq, int Nk, struct opnd Q, struct opnd K, struct opnd V,
+                  struct opnd O, hipb_mem qlen, hipb_mem klen, hipb_mem kmask,
+                  float scale, hipb_mem ws);
+/* Bytes of ws that cross_attend of this shape and HIPB_* type wants, or 0. */
+size_t cross_attend_ws(struct sam_model *m, int nb, int heads, int kv_heads,
+                       int hd, int Nq, int Nk, int dtype);
+
+/* Which columns of a head a pair is: (2j, 2j + 1), as rope_apply and the fused
+ * attention take them, or (j, j + rot / 2). */
+#define ROPE_PAIRS 0
+#define ROPE_HALVES 1
+
+/* How a table is scaled for contexts longer than the one trained on, by
+ * factor >= 1: not at all; positions divided by it (linear); theta times
+ * factor^(rot / (rot - 2)) (ntk); or (yarn) by parts: pairs that make
+ * beta_fast turns or more in the original context of orig positions stay,
+ * those with beta_slow or fewer are divided by factor, those between linearly
+ * between, and (cos, sin) are multiplied by 0.1 ln(factor) + 1. */
+#define ROPE_PLAIN 0
+#define ROPE_LINEAR 1
+#define ROPE_NTK 2
+#define ROPE_YARN 3
+struct rope_scale {
+    int kind;
+    double factor;
+    int orig;
+    double beta_fast, beta_slow;
+};
+
+/* Rotary table [npos][rot / 2] of float (cos, sin), as rope_apply, attn_fused,
+ * the model's rope_win / rope_glob and rope_rows read it: row p holds the
+ * angles of position pos[p] (int32; p itself where pos is NULL), position x
+ * theta^(-2j / rot) for pair j. Over a grid W tokens wide (W > 0) the first
+ * half of the pairs takes the position's column, the second its row, by
+ * theta^(-4j / rot), j < rot / 4, as SAM 3's trunk. Angles are reduced in 64
+ * bits. sc: scaling, or NULL; not for grids. */
+void rope_table(struct sam_model *m, hipb_mem table, int npos, hipb_mem pos,
+                int rot, int W, double theta, const struct rope_scale *sc);
+
+/* Rotates the first rot columns of rows of X by their position's table row
+ * into Y, and copies columns rot to hd: nb batches x heads of rows at off + b
+ * s0 + h s1 + r ld. Row r of batch b has position pos[b][r] (int32 [nb][rows]),
+ * or (pos0 + r) % npos where pos is NULL; a row whose position is outside 0 ..
+ * npos - 1 (-1, say) is not rotated. Y is X (in place) or does not overlap
+ * it; both have one element type. The inverse rotation (the gradient) is
+ * that of a table with the sines negated. */
+void rope_rows(struct sam_model *m, int nb, int heads, int rows, int hd,
+               int rot, int layout, struct opnd X, struct opnd Y,
+               hipb_mem table, int npos, hipb_mem pos, long pos0);
+
+#define ACT_SILU 3 /* x / (1 + exp(-x)): groupnorm only */
+
+/* Group norm of channels-last rows: nb batches (s0 apart; s1 is not used) of
+ * rows of C channels, mean and biased variance per batch and group of C /
+ * groups channels over all rows, y = act((x - mean) / sqrt(var + eps) g + b);
+ * g and b hold C floats (NULL: ones, zeros). Y may be X, or does not overlap
+ * it; both have one element type. ws as in cross_attend, groupnorm_ws bytes. */
+void groupnorm(struct sam_model *m, int nb, long rows, int C, int groups,
+               struct opnd X, struct opnd Y, hipb_mem g, hipb_mem b, float eps,
+               int act, hipb_mem ws);
+size_t groupnorm_ws(struct sam_model *m, int nb, long rows, int C, int groups,
+                    int dtype);
+
+/* ------------------------------------------------------------------ */
 /* Point-prompt mask decoder (sam3_model.c:1212-1517)                  */
 /* ------------------------------------------------------------------ */
 
