@@ -17,11 +17,13 @@
  * LDS (ds_read_b64_tr_b16); floats take v_mfma_f32_32x32x2, so that their
  * products are float products.
  *
- * Tiles of TK keys pass from memory through registers (loaded a tile ahead)
- * into LDS rows padded by 16 bytes, which leaves neither the 16-byte row reads
- * nor the transposed ones a bank conflict. Keys past the length and masked
- * keys enter LDS as zeros and their scores as minus infinity, so nothing that
- * stands in their memory reaches a result.
+ * Tiles of TK keys are copied straight into LDS (global_load_lds_dwordx4) a
+ * tile or more ahead of their use, the 16-byte chunks of a row swizzled so that
+ * neither the row reads of K nor the transposed reads of V meet a bank
+ * conflict. Operands whose rows do not start on 16 bytes take the same path
+ * through registers, element by element. Scores of keys past the length and
+ * of masked ones become minus infinity and their rows of V zeros, so nothing
+ * that stands in their memory reaches a result.
  */
 #include "k_common.h"
 
@@ -29,6 +31,13 @@ typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short i16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+struct yes {
+    static constexpr bool value = true;
+};
+struct no {
+    static constexpr bool value = false;
+};
 
 #define NEG_INF (-__builtin_inff())
 /* A row's maximum moves (and its sums are rescaled) when a score passes it
@@ -88,17 +97,17 @@ __device__ __forceinline__ f32x2 both_halves(float v)
     return o;
 }
 
-/* 16 bytes of a row at column byte cb: whole where vec, else element by
- * element, with zeros from column hd on. */
-template <int DT>
-__device__ __forceinline__ u32x4 row16(const char *p, int cb, int hdb, int vec)
+/* 16 bytes of a row at column byte cb: whole, or element by element, with
+ * zeros from column hd on. */
+template <int DT, bool VEC>
+__device__ __forceinline__ u32x4 row16(const char *p, int cb, int hdb)
 {
     constexpr int S = xt<DT>::size;
     u32x4 v = {0, 0, 0, 0};
 
     if (cb >= hdb)
         return v;
-    if (vec)
+    if (VEC)
         return *(const u32x4 *)(p + cb);
     if (S == 4) {
 #pragma unroll
@@ -115,7 +124,24 @@ __device__ __forceinline__ u32x4 row16(const char *p, int cb, int hdb, int vec)
     return v;
 }
 
-/* Four consecutive columns from c of output row p (S bytes each), c < hd. */
+/* One 16-byte step of S^T = K Q^T: the K row chunk at kp, Q's likewise. */
+template <int DT> __device__ __forceinline__ f32x16 k_step(const char *kp, u32x4 q, f32x16 s)
+{
+    const u32x4 k = *(const u32x4 *)kp;
+
+    if constexpr (DT == DT_F32) {
+        const f32x4 kx = __builtin_bit_cast(f32x4, k), qx = __builtin_bit_cast(f32x4, q);
+
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            s = __builtin_amdgcn_mfma_f32_32x32x2f32(kx[e], qx[e], s, 0, 0, 0);
+        return s;
+    }
+    else
+        return mfma16<DT>(k, q, s);
+}
+
+/* Column c of output row p. */
 template <int DT>
 __device__ __forceinline__ void put_elem(char *p, int c, float v)
 {
@@ -127,24 +153,86 @@ __device__ __forceinline__ void put_elem(char *p, int c, float v)
         ((_Float16 *)p)[c] = (_Float16)v;
 }
 
+/* Sixteen zeros: what stands for columns past the head width. */
+__device__ const u32x4 xattn_zeros = {0, 0, 0, 0};
+
+/* Layout of a tile's rows (RB bytes) in LDS. A copy fills 1 KiB, RPK rows; PAD
+ * bytes follow each. Chunk c (16 bytes) of row r stands in slot c ^ swz(r) of
+ * its row. LDS serves 256 bytes at once: K is read as one chunk of 32 rows,
+ * and 16 rows in turn take 16 different slots; V is read as 64 bytes of four
+ * rows (transposed, 16 bits) or 128 bytes of two rows four apart (floats),
+ * which take different quarters or halves. swz depends on r % RPK alone, and
+ * on few bits, so that an address is one of few registers and a constant. */
+template <int RB> struct row_k {
+    static constexpr int RPK = 1024 / RB;
+    static constexpr int PAD = RB == 64 ? 0 : RB <= 256 ? 64 : RB == 512 ? 32 : 16;
+    __device__ static __forceinline__ int swz(int r)
+    {
+        return RB == 64 ? r >> 2 & 3 : RB == 128 ? r >> 1 & 3 : RB == 256 ? r & 3 : RB == 512 ? r & 1 : 0;
+    }
+    __device__ static __forceinline__ int at(int r)
+    {
+        return r / RPK * (1024 + PAD) + r % RPK * RB;
+    }
+};
+template <int RB, int DT> struct row_v {
+    static constexpr int RPK = 1024 / RB;
+    static constexpr int PAD = DT == DT_F32 ? (RB == 256 ? 128 : RB == 512 ? 64 : RB == 1024 ? 32 : 0)
+                               : RB == 512 ? 128 : 0;
+    __device__ static __forceinline__ int swz(int r)
+    {
+        return DT == DT_F32 ? 0 : RB == 128 ? (r >> 1 & 1) << 2 : RB == 256 ? (r & 3) << 2 : RB == 512 ? (r & 1) << 2 : 0;
+    }
+    __device__ static __forceinline__ int at(int r)
+    {
+        return r / RPK * (1024 + PAD) + r % RPK * RB;
+    }
+};
+
+/* The same copy as g2lds16 from an address of each lane's own. */
+__device__ __forceinline__ void g2lds16_at(const void *src, unsigned lds)
+{
+    asm volatile("s_mov_b32 m0, %0\n\t"
+                 "s_nop 0\n\t"
+                 "global_load_lds_dwordx4 %1, off"
+                 :
+                 : "s"(lds), "v"(src)
+                 : "memory", "m0");
+}
+
+/* Waits until at most N of this wave's copies (the last issued) are under
+ * way, and for its LDS accesses, then for the workgroup. */
+template <int N> __device__ __forceinline__ void copies_and_barrier()
+{
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\t"
+                 "s_barrier"
+                 :
+                 : "n"(N)
+                 : "memory");
+}
+
 /* DP: head width padded to 32, 64, 128 or 256. WM waves share the rows of a
- * workgroup, 4 / WM the keys of a tile. TK: keys of a tile. */
-template <int DT, int DP, int WM, int TK>
-__global__ __launch_bounds__(256, DP == 256 || (DP == 128 && DT == DT_F32 && WM < 4) ? 1 : 2) void k_xattn(const struct xattn_desc a)
+ * workgroup, 4 / WM the keys of a tile. TK: keys of a tile. ST: tiles in LDS,
+ * ST - 1 of them ahead. VEC: the rows of all operands are whole 16-byte
+ * pieces. */
+template <int DT, int DP, int WM, int TK, int ST, int OCC, bool VEC>
+__global__ __launch_bounds__(256, OCC) void k_xattn(const struct xattn_desc a)
 {
     constexpr int S = xt<DT>::size;
     constexpr int WK = 4 / WM;
     constexpr int KW = TK / WK;          /* keys of a tile that a wave takes */
     constexpr int NB = KW / 32;          /* 32-key blocks of them */
-    constexpr int CH = DP * S / 16;      /* 16-byte chunks of a row */
-    constexpr int PITCH = DP * S + 16;
-    constexpr int NL = TK * CH / 256;    /* chunks per thread, K or V */
+    constexpr int RB = DP * S;           /* bytes of a row */
+    constexpr int CH = RB / 16;          /* 16-byte chunks of a row */
+    constexpr int NI = TK * RB / 4096;   /* copies of a wave for K or V: 1 KiB each */
     constexpr int MERGE = WK > 1 ? 4 * 32 * (DP + 4) * 4 + 4 * 32 * 8 : 0;
-    constexpr int TILES = 2 * TK * PITCH;
-    __shared__ __attribute__((aligned(16))) char lds[TILES > MERGE ? TILES : MERGE];
-    char *const ldk = lds, *const ldv = lds + TK * PITCH;
+    typedef row_k<RB> rk;
+    typedef row_v<RB, DT> rv;
+    constexpr int KT = TK / rk::RPK * (1024 + rk::PAD); /* LDS bytes of a tile's K */
+    constexpr int TILE = KT + TK / rv::RPK * (1024 + rv::PAD);
+    __shared__ __attribute__((aligned(1024))) char lds[ST * TILE > MERGE ? ST * TILE : MERGE];
 
-    static_assert(NL * 256 == TK * CH && KW % 32 == 0 && TK <= 128, "tile");
+    static_assert(NI >= 1 && KW % 32 == 0 && KW <= 64 && TK <= 128, "tile");
     const int tid = threadIdx.x, l = tid & 63;
     const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = l >> 5, lr = l & 31;
@@ -152,24 +240,27 @@ __global__ __launch_bounds__(256, DP == 256 || (DP == 128 && DT == DT_F32 && WM 
 
     /* Work item: XCD x (workgroup index mod 8) takes a contiguous range, so
      * that neighbours share its L2. */
-    const long per = (a.items + 7) / 8;
-    const long item = (long)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    const unsigned item = (blockIdx.x & 7) * ((a.items + 7) / 8) + (blockIdx.x >> 3);
 
-    if (item >= a.items || (long)(blockIdx.x >> 3) >= per)
+    if (item >= (unsigned)a.items)
         return;
-    int split, tile, unit;
+    unsigned split, tile, unit;
 
     if (a.heads_first) {
-        unit = (int)(item % a.units);
-        tile = (int)(item / a.units % a.tiles);
-        split = (int)(item / a.units / a.tiles);
+        const unsigned rest = item / a.units;
+
+        unit = item - rest * a.units;
+        split = rest / a.tiles;
+        tile = rest - split * a.tiles;
     }
     else {
-        tile = (int)(item % a.tiles);
-        split = (int)(item / a.tiles % a.splits);
-        unit = (int)(item / a.tiles / a.splits);
+        const unsigned rest = item / a.tiles;
+
+        tile = item - rest * a.tiles;
+        unit = rest / a.splits;
+        split = rest - unit * a.splits;
     }
-    const int b = unit / a.kvh, kh = unit % a.kvh;
+    const int b = unit / (unsigned)a.kvh, kh = unit - b * a.kvh;
     const int nq = a.qlen ? max(0, min(a.qlen[b], a.Nq)) : a.Nq;
     const int nk = a.klen ? max(0, min(a.klen[b], a.Nk)) : a.Nk;
     const int rows = a.grp * nq;
@@ -181,11 +272,73 @@ __global__ __launch_bounds__(256, DP == 256 || (DP == 128 && DT == DT_F32 && WM 
     const int jb = min(nk, split * per_split), je = min(nk, jb + per_split);
     const int hdb = a.hd * S;
 
+    const char *const kb = (const char *)a.K + S * (a.ko + (long)b * a.ks0 + (long)kh * a.ks1);
+    const char *const vb = (const char *)a.V + S * (a.vo + (long)b * a.vs0 + (long)kh * a.vs1);
+    const uint8_t *const mk = a.kmask ? a.kmask + (long)b * a.Nk : nullptr;
+    const uint32_t kstep = (uint32_t)a.kld * S, vstep = (uint32_t)a.vld * S;
+
+    /* Copy i of this wave fills rows (w NI + i) RPK on of a tile; lane l's 16
+     * bytes are of row l / CH of them. koff, voff: their offsets in memory from
+     * the copy's first row. lk, lv: where the wave's copies go in slot 0. */
+    const int lrow = l / CH;
+    const int ck = 16 * ((l % CH) ^ rk::swz(lrow)), cv = 16 * ((l % CH) ^ rv::swz(lrow));
+    const uint32_t koff = lrow * kstep + ck, voff = lrow * vstep + cv;
+    const unsigned lk = (unsigned)(uintptr_t)lds + w * NI * (1024 + rk::PAD);
+    const unsigned lv = (unsigned)(uintptr_t)lds + KT + w * NI * (1024 + rv::PAD);
+    /* Starts the copies of a tile of which every row is whole, from rows kt and
+     * vt (the wave's first) into slot st. */
+    auto copy_full = [&](const char *kt, const char *vt, int st) {
+        const unsigned tk = __builtin_amdgcn_readfirstlane(lk + st * TILE);
+        const unsigned tv = __builtin_amdgcn_readfirstlane(lv + st * TILE);
+
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            g2lds16(kt + (long)(i * rk::RPK) * kstep, koff, tk + (1024 + rk::PAD) * i);
+            g2lds16(vt + (long)(i * rv::RPK) * vstep, voff, tv + (1024 + rv::PAD) * i);
+        }
+    };
+    /* The tile at key j0, up to key je (its last row stands for those behind)
+     * and column hd (zeros behind). */
+    auto copy = [&](int j0, int st) {
+        const int last = je - 1 - j0, w0 = w * NI * rk::RPK;
+
+        if (VEC && a.hd == DP && last >= TK - 1) {
+            copy_full(kb + (long)(j0 + w0) * kstep, vb + (long)(j0 + w0) * vstep, st);
+            return;
+        }
+        const unsigned tk = __builtin_amdgcn_readfirstlane(lk + st * TILE);
+        const unsigned tv = __builtin_amdgcn_readfirstlane(lv + st * TILE);
+
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const int rr = j0 + min(w0 + i * rk::RPK + lrow, last);
+            const char *pk = kb + (long)rr * kstep, *pv = vb + (long)rr * vstep;
+
+            if (VEC) {
+                g2lds16_at(ck < hdb ? pk + ck : (const char *)&xattn_zeros,
+                           tk + (1024 + rk::PAD) * i);
+                g2lds16_at(cv < hdb ? pv + cv : (const char *)&xattn_zeros,
+                           tv + (1024 + rv::PAD) * i);
+            }
+            else {
+                char *const at = lds + st * TILE + 16 * l;
+
+                *(u32x4 *)(at + (w * NI + i) * (1024 + rk::PAD)) = row16<DT, VEC>(pk, ck, hdb);
+                *(u32x4 *)(at + KT + (w * NI + i) * (1024 + rv::PAD)) =
+                    row16<DT, VEC>(pv, cv, hdb);
+            }
+        }
+    };
+
+    /* The first tiles, on their way while Q is read. */
+#pragma unroll
+    for (int i = 0; i < ST - 1; i++)
+        if (jb + i * TK < je)
+            copy(jb + i * TK, i);
     /* This lane's row: query and head, and its part of Q. */
     const int r = r0 + wm * 32 + lr;
     const int rc = min(r, rows - 1);
-    const int hq = rc / nq, iq = rc % nq;
-    const long orow = a.oo + (long)b * a.os0 + (long)(kh * a.grp + hq) * a.os1 + (long)iq * a.old;
+    const int hq = a.grp == 1 ? 0 : rc / nq, iq = rc - hq * nq;
     u32x4 qf[CH / 2];
     {
         const char *q = (const char *)a.Q +
@@ -194,97 +347,47 @@ __global__ __launch_bounds__(256, DP == 256 || (DP == 128 && DT == DT_F32 && WM 
 
 #pragma unroll
         for (int i = 0; i < CH / 2; i++)
-            qf[i] = row16<DT>(q, 16 * (2 * i + h), hdb, a.qvec);
+            qf[i] = row16<DT, VEC>(q, 16 * (2 * i + h), hdb);
     }
-    const char *kb = (const char *)a.K + S * (a.ko + (long)b * a.ks0 + (long)kh * a.ks1);
-    const char *vb = (const char *)a.V + S * (a.vo + (long)b * a.vs0 + (long)kh * a.vs1);
-    const uint8_t *mk = a.kmask ? a.kmask + (long)b * a.Nk : nullptr;
-    const uint32_t kstep = (uint32_t)a.kld * S, vstep = (uint32_t)a.vld * S;
-
-    u32x4 sk[NL], sv[NL];
-    auto load = [&](int j0) {
-        const char *kt = kb + (long)j0 * kstep, *vt = vb + (long)j0 * vstep;
-        const int last = je - 1 - j0;
-
+    /* Q has arrived: left to its first use, the wait for it would stand inside
+     * the loop and wait for the copies of the next tile there each time. */
 #pragma unroll
-        for (int i = 0; i < NL; i++) {
-            const int c = tid + 256 * i, row = c / CH, cb = c % CH * 16;
-            const int rr = min(row, last);
-
-            sk[i] = row16<DT>(kt + (uint32_t)rr * kstep, cb, hdb, a.kvec);
-            sv[i] = row16<DT>(vt + (uint32_t)rr * vstep, cb, hdb, a.vvec);
-        }
-        if (mk || last < TK - 1) {
-#pragma unroll
-            for (int i = 0; i < NL; i++) {
-                const int row = (tid + 256 * i) / CH;
-                const bool ok = row <= last && (!mk || mk[j0 + min(row, last)]);
-
-                if (!ok)
-                    sk[i] = sv[i] = u32x4{0, 0, 0, 0};
-            }
-        }
-    };
-    auto store = [&]() {
-#pragma unroll
-        for (int i = 0; i < NL; i++) {
-            const int c = tid + 256 * i, row = c / CH, cb = c % CH * 16;
-
-            *(u32x4 *)(ldk + row * PITCH + cb) = sk[i];
-            *(u32x4 *)(ldv + row * PITCH + cb) = sv[i];
-        }
-    };
-
+    for (int i = 0; i < CH / 2; i++)
+        asm volatile("" : "+v"(qf[i]));
     f32x16 o[DP / 32];
     float m = NEG_INF, sum = 0.0f;
 
 #pragma unroll
     for (int i = 0; i < DP / 32; i++)
         o[i] = f32x16{0};
-    if (jb < je)
-        load(jb);
-    for (int j0 = jb; j0 < je; j0 += TK) {
-        __syncthreads();
-        store();
-        __syncthreads();
-        /* Which of this wave's keys count, a bit for each. */
-        uint64_t keep;
-        {
-            const int j = j0 + wk * KW + l;
-            bool ok = l < KW && j < je;
-
-            if (mk)
-                ok = ok && mk[min(j, je - 1)] != 0;
-            keep = __ballot(ok);
-        }
-        if (j0 + TK < je)
-            load(j0 + TK);
-        if (keep == 0)
-            continue;
+    /* This wave's keys of the tile in slot st: all of them, or those whose
+     * bit in keep is set. */
+    auto attend_tile = [&](auto all, int st, uint64_t keep) {
+        constexpr bool ALL = decltype(all)::value;
+        char *const ldk = lds + st * TILE + wk * rk::at(KW);
+        char *const ldv = lds + st * TILE + KT + wk * rv::at(KW);
+        /* The second block of 32 keys is empty. */
+        const bool half = !ALL && NB == 2 && keep >> 32 == 0;
         f32x16 s[NB];
 
 #pragma unroll
-        for (int n = 0; n < NB; n++) {
-            const char *kr = ldk + (wk * KW + n * 32 + lr) * PITCH + 16 * h;
-
+        for (int n = 0; n < NB; n++)
             s[n] = f32x16{0};
+        if (half) {
 #pragma unroll
-            for (int i = 0; i < CH / 2; i++) {
-                const u32x4 kf = *(const u32x4 *)(kr + 32 * i);
-
-                if constexpr (DT == DT_F32) {
-                    const f32x4 kx = __builtin_bit_cast(f32x4, kf);
-                    const f32x4 qx = __builtin_bit_cast(f32x4, qf[i]);
-
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        s[n] = __builtin_amdgcn_mfma_f32_32x32x2f32(kx[e], qx[e], s[n], 0, 0, 0);
-                }
-                else
-                    s[n] = mfma16<DT>(kf, qf[i], s[n]);
-            }
+            for (int i = 0; i < CH / 2; i++)
+                s[0] = k_step<DT>(ldk + rk::at(lr) + 16 * ((2 * i + h) ^ rk::swz(lr)), qf[i], s[0]);
         }
-        if (KW == 64 ? ~keep != 0 : (uint32_t)keep != 0xffffffffu) {
+        else {
+#pragma unroll
+            for (int i = 0; i < CH / 2; i++)
+#pragma unroll
+                for (int n = 0; n < NB; n++)
+                    s[n] = k_step<DT>(ldk + rk::at(n * 32) + rk::at(lr) +
+                                          16 * ((2 * i + h) ^ rk::swz(lr)),
+                                      qf[i], s[n]);
+        }
+        if (!ALL && (KW == 64 ? ~keep != 0 : (uint32_t)keep != 0xffffffffu)) {
 #pragma unroll
             for (int n = 0; n < NB; n++) {
                 const uint32_t bits = (uint32_t)(keep >> (32 * n)) >> (4 * h);
@@ -294,6 +397,10 @@ __global__ __launch_bounds__(256, DP == 256 || (DP == 128 && DT == DT_F32 && WM 
                     if (!(bits >> (8 * (i / 4) + i % 4) & 1))
                         s[n][i] = NEG_INF;
             }
+            /* Their rows of V, by each wave that reads them. */
+            for (int c = l; c < KW * CH; c += 64)
+                if (!(keep >> (c / CH) & 1))
+                    *(u32x4 *)(ldv + rv::at(c / CH) + 16 * (c % CH)) = u32x4{0, 0, 0, 0};
         }
         float mx = s[0][0];
 
@@ -321,23 +428,24 @@ __global__ __launch_bounds__(256, DP == 256 || (DP == 128 && DT == DT_F32 && WM 
 
 #pragma unroll
         for (int n = 0; n < NB; n++) {
-            float t[4] = {0, 0, 0, 0};
+            float t[4];
 
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], a.c, -ref));
-                t[i & 3] += s[n][i];
+                t[i & 3] = i < 4 ? s[n][i] : t[i & 3] + s[n][i];
             }
             sum += (t[0] + t[1]) + (t[2] + t[3]);
         }
 #pragma unroll
         for (int n = 0; n < NB; n++) {
+            if (n && half)
+                break;
             if constexpr (DT == DT_F32) {
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const char *vr = ldv +
-                                     (wk * KW + n * 32 + 8 * (i / 4) + i % 4 + 4 * h) * PITCH +
-                                     4 * lr;
+                    const char *vr =
+                        ldv + rv::at(n * 32 + 8 * (i / 4)) + rv::at(i % 4 + 4 * h) + 4 * lr;
 
 #pragma unroll
                     for (int d = 0; d < DP / 32; d++)
@@ -347,18 +455,19 @@ __global__ __launch_bounds__(256, DP == 256 || (DP == 128 && DT == DT_F32 && WM 
             }
             else {
 #pragma unroll
-                for (int st = 0; st < 2; st++) {
-                    const char *vr = ldv +
-                                     (wk * KW + n * 32 + 16 * st + 4 * h + (l & 15) / 4) * PITCH +
-                                     32 * (l >> 4 & 1) + 8 * (l & 3);
+                for (int hf = 0; hf < 2; hf++) {
+                    const int row = 4 * h + (l & 15) / 4;
+                    const char *vr = ldv + rv::at(n * 32 + 16 * hf) + rv::at(row) + 8 * (l & 1);
+                    const int c0 = 2 * (l >> 4 & 1) + (l >> 1 & 1);
                     u32x4 p;
 
 #pragma unroll
                     for (int i = 0; i < 4; i++)
-                        p[i] = pack2<DT>(s[n][8 * st + 2 * i], s[n][8 * st + 2 * i + 1]);
+                        p[i] = pack2<DT>(s[n][8 * hf + 2 * i], s[n][8 * hf + 2 * i + 1]);
 #pragma unroll
                     for (int d = 0; d < DP / 32; d++) {
-                        const u32x2 v0 = lds_tr(vr + 64 * d), v1 = lds_tr(vr + 8 * PITCH + 64 * d);
+                        const char *vd = vr + 16 * ((4 * d + c0) ^ rv::swz(row));
+                        const u32x2 v0 = lds_tr(vd), v1 = lds_tr(vd + rv::at(8));
                         const u32x4 vf = {v0.x, v0.y, v1.x, v1.y};
 
                         o[d] = mfma16<DT>(vf, p, o[d]);
@@ -366,6 +475,39 @@ __global__ __launch_bounds__(256, DP == 256 || (DP == 128 && DT == DT_F32 && WM 
                 }
             }
         }
+    };
+    int j0 = jb, st = 0;
+
+    /* Whole tiles whose copies ahead are whole tiles too: nothing to check. */
+    if (VEC && a.hd == DP && !mk) {
+        const long ahead = j0 + (ST - 1) * TK + w * NI * rk::RPK;
+        const char *kt = kb + ahead * kstep, *vt = vb + ahead * vstep;
+
+        for (; j0 + ST * TK <= je; j0 += TK) {
+            copies_and_barrier<(ST - 2) * 2 * NI>();
+            copy_full(kt, vt, st == 0 ? ST - 1 : st - 1);
+            kt += (long)TK * kstep;
+            vt += (long)TK * vstep;
+            attend_tile(yes{}, st, 0);
+            st = st + 1 == ST ? 0 : st + 1;
+        }
+    }
+    for (; j0 < je; j0 += TK, st = st + 1 == ST ? 0 : st + 1) {
+        const int j = min(j0 + wk * KW + (l & (KW - 1)), je - 1);
+        const bool drop = mk && mk[j] == 0;
+
+        /* This tile has landed, and the slot of the one before is free. */
+        if (ST > 2 && j0 + (ST - 2) * TK < je)
+            copies_and_barrier<(ST - 2) * 2 * NI>();
+        else
+            copies_and_barrier<0>();
+        if (j0 + (ST - 1) * TK < je)
+            copy(j0 + (ST - 1) * TK, st == 0 ? ST - 1 : st - 1);
+        /* Which of this wave's keys count. */
+        const uint64_t keep = __ballot(l < KW && j0 + wk * KW + l < je && !drop);
+
+        if (keep)
+            attend_tile(no{}, st, keep);
     }
     /* The two halves of a row's sum. */
     const f32x2 sh = both_halves(sum);
@@ -446,7 +588,7 @@ __global__ __launch_bounds__(256, DP == 256 || (DP == 128 && DT == DT_F32 && WM 
                     for (int q = 0; q < 4; q++) {
                         const int c = 32 * d + 8 * q + 4 * h;
 
-                        if (a.pvec) {
+                        if (VEC) {
                             if (c < a.hd)
                                 *(f32x4 *)(rec + c) = f32x4{o[d][4 * q], o[d][4 * q + 1],
                                                             o[d][4 * q + 2], o[d][4 * q + 3]};
@@ -461,7 +603,8 @@ __global__ __launch_bounds__(256, DP == 256 || (DP == 128 && DT == DT_F32 && WM 
         return;
     }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    char *const op = (char *)a.O + S * orow;
+    char *const op = (char *)a.O + S * (a.oo + (long)b * a.os0 + (long)(kh * a.grp + hq) * a.os1 +
+                                        (long)iq * a.old);
 
 #pragma unroll
     for (int d = 0; d < DP / 32; d++) {
@@ -476,7 +619,7 @@ __global__ __launch_bounds__(256, DP == 256 || (DP == 128 && DT == DT_F32 && WM 
                 x[e] = o[d][4 * q + e] * inv;
             const int c = 32 * d + 8 * q;
 
-            if (!a.ovec) {
+            if constexpr (!VEC) {
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     const int ce = c + 8 * (e / 4) + 4 * h + e % 4;
@@ -506,49 +649,85 @@ __global__ __launch_bounds__(256, DP == 256 || (DP == 128 && DT == DT_F32 && WM 
     }
 }
 
-/* The splits of a row, a wave each: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s -
- * M) l_s with M the largest m_s. */
-template <int DT>
+/* The splits of a row: o = sum_s 2^(m_s - M) O_s / sum_s 2^(m_s - M) l_s, M the
+ * largest m_s. LP lanes per row, four columns each (or one where rows are no
+ * multiple of four), eight splits' loads under way at a time. */
+template <int DT, int LP, bool VEC>
 __global__ __launch_bounds__(256) void k_xattn_merge(const struct xattn_desc a)
 {
-    const long ur = (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    constexpr int V = VEC ? 4 : 1;
+    const int lane = threadIdx.x % LP;
+    const long ur = (long)blockIdx.x * (256 / LP) + threadIdx.x / LP;
     const long nrow = (long)a.grp * a.Nq, total = nrow * a.units;
-    const int l = threadIdx.x & 63;
 
     if (ur >= total)
         return;
-    const int unit = (int)(ur / nrow), r = (int)(ur % nrow);
+    const int unit = (int)(ur / nrow), r = (int)(ur - unit * nrow);
     const int b = unit / a.kvh, kh = unit % a.kvh;
     const int nq = a.qlen ? max(0, min(a.qlen[b], a.Nq)) : a.Nq;
 
     if (r >= a.grp * nq)
         return;
     const float2 *ml = (const float2 *)(a.part + a.part_ml) + ur;
-    float m = NEG_INF, sum = 0.0f;
-
-    for (int s = 0; s < a.splits; s++)
-        m = fmaxf(m, ml[s * total].x);
-    const float ref = m == NEG_INF ? 0.0f : m;
-
-    for (int s = 0; s < a.splits; s++)
-        sum += ml[s * total].y * __builtin_amdgcn_exp2f(ml[s * total].x - ref);
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     char *const op = (char *)a.O +
                      (long)xt<DT>::size * (a.oo + (long)b * a.os0 +
                                            (long)(kh * a.grp + r / nq) * a.os1 +
                                            (long)(r % nq) * a.old);
 
-    for (int c = l; c < a.hd; c += 64) {
-        float o = 0.0f;
+    for (int c = lane * V; c < a.hd; c += LP * V) {
+        const float *const rec = a.part + ur * a.hd + c;
+        float m = NEG_INF, sum = 0.0f, o[V] = {0};
 
-        for (int s = 0; s < a.splits; s++) {
-            const float2 x = ml[s * total];
+        for (int s0 = 0; s0 < a.splits; s0 += 8) {
+            float2 x[8];
+            float v[8][V];
+            float mn = m;
 
-            /* A split without keys left no sums. */
-            if (x.y != 0.0f)
-                o += a.part[(ur + s * total) * a.hd + c] * __builtin_amdgcn_exp2f(x.x - ref);
+#pragma unroll
+            for (int k = 0; k < 8; k++) {
+                const int s = min(s0 + k, a.splits - 1);
+
+                x[k] = ml[s * total];
+                if constexpr (VEC)
+                    *(f32x4 *)v[k] = *(const f32x4 *)(rec + s * total * a.hd);
+                else
+                    v[k][0] = rec[s * total * a.hd];
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (s0 + k < a.splits)
+                    mn = fmaxf(mn, x[k].x);
+            const float ref = mn == NEG_INF ? 0.0f : mn;
+            const float f = __builtin_amdgcn_exp2f(m - ref);
+
+            m = mn;
+            sum *= f;
+#pragma unroll
+            for (int e = 0; e < V; e++)
+                o[e] *= f;
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                /* A split without keys left no sums. */
+                if (s0 + k < a.splits && x[k].y != 0.0f) {
+                    const float g = __builtin_amdgcn_exp2f(x[k].x - ref);
+
+                    sum = fmaf(g, x[k].y, sum);
+#pragma unroll
+                    for (int e = 0; e < V; e++)
+                        o[e] = fmaf(g, v[k][e], o[e]);
+                }
         }
-        put_elem<DT>(op, c, o * inv);
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+
+#pragma unroll
+        for (int e = 0; e < V; e++)
+            o[e] *= inv;
+        if constexpr (!VEC)
+            put_elem<DT>(op, c, o[0]);
+        else if constexpr (DT == DT_F32)
+            *(f32x4 *)(op + 4 * c) = f32x4{o[0], o[1], o[2], o[3]};
+        else
+            *(u32x2 *)(op + 2 * c) = u32x2{pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3])};
     }
 }
 
@@ -560,37 +739,61 @@ static int padded(int hd)
     return hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
 }
 
-/* Rows of 32 of a workgroup (the rest of its four waves split the keys) and
- * the key splits. Sets wm and splits of the problem. */
+/* How the work is cut. A workgroup of wm x 32 rows walks all keys of its rows,
+ * or one of several splits of them whose sums a second launch adds up. More rows
+ * share each copied tile; fewer make more workgroups, whose waves then share
+ * the keys. us on 256 compute units, f16 but for the last, wm 4 / 2 / 1:
+ *   12 heads of 64, 447 rows, 1500 keys: batch 64 207 / 217 / 367, batch 4 22.8 /
+ *   21.3 / 23.3, batch 1 - / 16.0 / 11.7 (15.0 with two splits of wm 1);
+ *   8 heads of 64, 1000 x 1000: 16.5 / 12.4 / 9.7 (best split 14.5);
+ *   one head of 256, 5184 x 20751, bf16: 144 with 12 splits, 192 with 16 (a
+ *   workgroup too many per compute unit), 175 with 8, wm 2 236.
+ * So: as many rows as still give two workgroups per compute unit, or one and a
+ * quarter with wm 2; splits only where even the least rows leave half of the
+ * compute units idle, and then two workgroups for each.
+ * With few rows the splits' sums are small, and lengths may differ: 16
+ * sequences of 40 to 100 % of 8192 keys, 8 key heads of 128: 79 us with eight
+ * splits, 89 with four, 83 with sixteen (four workgroups per compute unit);
+ * but 64 sequences of 2048 67 without and 75 with two. */
 static void plan(struct xattn_desc *d)
 {
-    const int cu = dev_cu_count();
-    const long rows = (long)d->grp * d->Nq;
-    long wg;
+    const long cu = dev_cu_count(), rows = (long)d->grp * d->Nq;
+    const int rb = padded(d->hd) * (d->dt == DT_F32 ? 4 : 2);
+    /* Waves that share keys have 32 of a tile each: wider rows would leave LDS
+     * for one workgroup per compute unit (step of 16 sequences above: wm 1 88
+     * us, wm 2 79), or none. */
+    const int least = rb >= 1024 ? 4 : rb >= 256 ? 2 : 1;
     int wm = rows > 64 ? 4 : rows > 32 ? 2 : 1;
 
-    if (wm == 1 && d->dt == DT_F32 && padded(d->hd) == 256)
-        wm = 2;
-    while (wm > 1 && !(wm == 2 && d->dt == DT_F32 && padded(d->hd) == 256) &&
-           (long)d->units * ((rows + 32 * wm - 1) / (32 * wm)) < cu && d->Nk > 64 * 4 / wm)
-        wm /= 2;
+#define WG(wm) (d->units * ((rows + 32 * (wm) - 1) / (32 * (wm))))
+    if (wm < least)
+        wm = least;
+    d->splits = 1;
+    if (!d->vec)
+        wm = rb >= 1024 ? 4 : 2;
+    else if (d->Nk > 256) {
+        const int most_rows = wm;
+        long want = 2 * cu;
+
+        if (wm == 4 && least <= 2 && WG(4) < 2 * cu)
+            wm = 2;
+        if (wm == 2 && least == 1 && WG(2) < cu + cu / 4)
+            wm = 1;
+        if (rows <= 64 ? WG(wm) < 2 * cu : WG(wm) <= cu / 2) {
+            wm = most_rows;
+            if (rows <= 64)
+                want = 4 * cu;
+            want /= WG(wm);
+            if (want > d->Nk / 384)
+                want = d->Nk / 384;
+            d->splits = want < 1 ? 1 : want > 64 ? 64 : (int)want;
+        }
+    }
     d->wm = wm;
     d->tiles = (int)((rows + 32 * wm - 1) / (32 * wm));
-    wg = (long)d->units * d->tiles;
-    d->splits = 1;
-    if (wg < 2 * cu) {
-        const long most = d->Nk / (wm == 1 ? 256 : 128);
-
-        d->splits = (int)((2 * cu + wg - 1) / wg);
-        if (d->splits > most)
-            d->splits = (int)most;
-        if (d->splits > 64)
-            d->splits = 64;
-        if (d->splits < 1)
-            d->splits = 1;
-    }
-    d->items = wg * d->splits;
+    d->items = WG(wm) * d->splits;
     d->heads_first = d->Nk <= 256;
+#undef WG
 }
 
 /* Offset of the splits' (m, sum) pairs in floats, and all of the workspace
@@ -608,26 +811,55 @@ extern "C" size_t xattn_ws(struct xattn_desc *d)
     return 4 * part_ml(d) + 8 * (size_t)d->splits * d->units * d->grp * d->Nq;
 }
 
-template <int DT, int DP, int WM, int TK>
+template <int DT, int DP, int WM, int TK, int ST, int OCC, bool VEC = true>
 static int run(const struct xattn_desc *d, hipStream_t s)
 {
     const long grid = (d->items + 7) / 8 * 8;
 
-    hipLaunchKernelGGL((k_xattn<DT, DP, WM, TK>), dim3((unsigned)grid), dim3(256), 0, s, *d);
+    hipLaunchKernelGGL((k_xattn<DT, DP, WM, TK, ST, OCC, VEC>), dim3((unsigned)grid), dim3(256), 0,
+                       s, *d);
     return hipGetLastError();
 }
 
 template <int DT, int DP> static int run_wm(const struct xattn_desc *d, hipStream_t s)
 {
-    constexpr bool wide = DP * xt<DT>::size >= 512;
+    constexpr int RB = DP * xt<DT>::size;
 
-    if (d->wm == 4)
-        return run<DT, DP, 4, wide ? 32 : 64>(d, s);
-    if (d->wm == 2)
-        return run<DT, DP, 2, 64>(d, s);
-    if constexpr (DP * xt<DT>::size <= 512)
-        return run<DT, DP, 1, 128>(d, s);
+    if (!d->vec) {
+        if constexpr (RB == 1024)
+            return run<DT, DP, 4, 32, 2, 1, false>(d, s);
+        else
+            return run<DT, DP, 2, 64, 2, 1, false>(d, s);
+    }
+    /* LDS of a tile of 64 keys: 8, 16, 32 KiB for rows of 64, 128, 256 bytes. */
+    if (d->wm == 4) {
+        if constexpr (RB <= 128)
+            return run<DT, DP, 4, 64, 3, 2>(d, s);
+        else if constexpr (RB == 256)
+            return run<DT, DP, 4, 64, 2, 2>(d, s);
+        else if constexpr (RB == 512)
+            return run<DT, DP, 4, 32, 2, 2>(d, s);
+        else
+            return run<DT, DP, 4, 32, 2, 1>(d, s);
+    }
+    if (d->wm == 2) {
+        if constexpr (RB <= 256)
+            return run<DT, DP, 2, 64, 2, 2>(d, s);
+        else if constexpr (RB == 512)
+            return run<DT, DP, 2, 64, 2, 1>(d, s);
+    }
+    if constexpr (RB <= 128)
+        return run<DT, DP, 1, 128, 2, 2>(d, s);
+    else if constexpr (RB == 256)
+        return run<DT, DP, 1, 128, 2, 1>(d, s);
     return hipErrorInvalidValue;
+}
+
+template <int DT, int LP, bool VEC> static void merge(const struct xattn_desc *d, hipStream_t s)
+{
+    const long rows = (long)d->units * d->grp * d->Nq, blocks = (rows * LP + 255) / 256;
+
+    hipLaunchKernelGGL((k_xattn_merge<DT, LP, VEC>), dim3((unsigned)blocks), dim3(256), 0, s, *d);
 }
 
 template <int DT> static int run_dt(struct xattn_desc *d, hipStream_t s)
@@ -639,10 +871,12 @@ template <int DT> static int run_dt(struct xattn_desc *d, hipStream_t s)
                           : run_wm<DT, 256>(d, s);
 
     if (err == hipSuccess && d->splits > 1) {
-        const long rows = (long)d->units * d->grp * d->Nq;
-
-        hipLaunchKernelGGL((k_xattn_merge<DT>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, s,
-                           *d);
+        if (!d->vec)
+            merge<DT, 64, false>(d, s);
+        else if (dp <= 64)
+            merge<DT, 16, true>(d, s);
+        else
+            merge<DT, 32, true>(d, s);
         err = hipGetLastError();
     }
     return err;

@@ -353,12 +353,12 @@ struct xattn_desc {
     void *O;
     long qo, qs0, qs1, ko, ks0, ks1, vo, vs0, vs1, oo, os0, os1;
     int qld, kld, vld, old;
-    int qvec, kvec, vvec, ovec; /* 16-byte accesses of whole rows fit */
+    int vec; /* rows of all four are whole 16-byte pieces */
     const int *qlen, *klen;
     const unsigned char *kmask;
     int units, kvh, grp, hd, Nq, Nk, dt;
     float c; /* scale log2 e */
-    int wm, tiles, splits, heads_first, pvec;
+    int wm, tiles, splits, heads_first;
     long items;
     float *part; /* [split][unit][grp Nq] rows of hd sums, then (m, sum) */
     long part_ml;

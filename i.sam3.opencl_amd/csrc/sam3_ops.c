@@ -1739,11 +1739,16 @@ size_t cross_attend_ws(struct sam_model *m, int nb, int heads, int kv_heads, int
                        int Nk, int dtype)
 {
     struct xattn_desc d;
+    size_t n;
 
     if (!xattn_shape(&d, "cross_attend_ws", nb, heads, kv_heads, hd, Nq, Nk, dtype) || nb == 0 ||
         Nq == 0)
         return 0;
-    return xattn_ws(&d);
+    /* Whatever the operands' alignment. */
+    d.vec = 1;
+    n = xattn_ws(&d);
+    d.vec = 0;
+    return xattn_ws(&d) > n ? xattn_ws(&d) : n;
 }
 
 void cross_attend(struct sam_model *m, int nb, int heads, int kv_heads, int hd, int Nq, int Nk,
@@ -1800,6 +1805,9 @@ void cross_attend(struct sam_model *m, int nb, int heads, int kv_heads, int hd, 
         (klen && !bytes_ok(op, "klen", klen, 4 * (size_t)nb)) ||
         (kmask && !bytes_ok(op, "kmask", kmask, (size_t)nb * Nk)))
         return;
+    d.vec = hd * elem_size(d.dt) % 16 == 0 && opnd_vec(Q, nb, heads, Nq) &&
+            opnd_vec(K, nb, kv_heads, Nk) && opnd_vec(V, nb, kv_heads, Nk) &&
+            opnd_vec(O, nb, heads, Nq);
     need = xattn_ws(&d);
     if (!workspace(be, op, ws, need, &wp, &ws_bytes))
         return;
@@ -1823,12 +1831,6 @@ void cross_attend(struct sam_model *m, int nb, int heads, int kv_heads, int hd, 
     d.os0 = O.s0;
     d.os1 = O.s1;
     d.old = O.ld;
-    i = hd * elem_size(d.dt) % 16 == 0;
-    d.qvec = i && opnd_vec(Q, nb, heads, Nq);
-    d.kvec = i && opnd_vec(K, nb, kv_heads, Nk);
-    d.vvec = i && opnd_vec(V, nb, kv_heads, Nk);
-    d.ovec = i && opnd_vec(O, nb, heads, Nq);
-    d.pvec = hd % 4 == 0;
     d.qlen = qlen ? qlen->ptr : NULL;
     d.klen = klen ? klen->ptr : NULL;
     d.kmask = kmask ? kmask->ptr : NULL;
