@@ -13,84 +13,110 @@
 #include "k_common.h"
 
 #define ACT_SILU_K 3
+/* Threads of the kernels that share a batch entry's rows, and vectors that each
+ * has under way. us of both kernels at 82944 rows of 256 floats: 512 threads,
+ * two workgroups per compute unit for the sums, one for the rest 17.4 + 28.3;
+ * 256 threads and four 15.8 + 37; 1024 and one 20.0 + 28.5 (every workgroup of
+ * the second kernel adds up all sums of its batch entry). */
+#define TH 512
+#define AHEAD_SUMS 4
+#define AHEAD_APPLY 8
+/* Elements of a group that one workgroup takes, where a row's part of the
+ * group is at least 16 bytes, and below that, where it reads lines for few
+ * bytes of them. us by one workgroup per group and split: 8 groups of 32
+ * halves, 400 rows 7.0 and 12.3, 1000 rows 13.0 and 13.2; 32 groups of 10
+ * floats, 1200 rows 8.9 and 14.6; 256 groups of one float, 5000 rows 59 and
+ * 23. */
+#define SPLIT_ABOVE (16 * 1024)
+#define SPLIT_ABOVE_NARROW (4 * 1024)
 
 template <int DT> __device__ __forceinline__ float from(uint16_t v)
 {
     return DT == DT_BF16 ? bf2f(v) : h2f(v);
 }
 
-/* V consecutive elements as floats, and back. */
+template <int BYTES> struct raw_of;
+template <> struct raw_of<16> {
+    typedef u32x4 type;
+};
+template <> struct raw_of<8> {
+    typedef u32x2 type;
+};
+template <> struct raw_of<4> {
+    typedef uint32_t type;
+};
+template <> struct raw_of<2> {
+    typedef uint16_t type;
+};
+
+/* V consecutive elements as they are stored, and as floats. */
 template <int DT, int V> struct vec {
+    static constexpr int size = DT == DT_F32 ? 4 : 2;
+    typedef typename raw_of<V * size>::type raw;
     float v[V];
 
-    __device__ __forceinline__ void get(const void *base, long at)
+    __device__ __forceinline__ void set(raw r)
     {
-        if constexpr (DT == DT_F32) {
-            const float *p = (const float *)base + at;
-
-            if constexpr (V == 4)
-                *(f32x4 *)v = *(const f32x4 *)p;
-            else if constexpr (V == 2)
-                *(float2 *)v = *(const float2 *)p;
-            else
-                v[0] = p[0];
-        }
+        if constexpr (DT == DT_F32)
+            __builtin_memcpy(v, &r, sizeof r);
         else {
-            const uint16_t *p = (const uint16_t *)base + at;
             uint16_t u[V];
 
-            if constexpr (V == 8)
-                *(u32x4 *)u = *(const u32x4 *)p;
-            else if constexpr (V == 4)
-                *(u32x2 *)u = *(const u32x2 *)p;
-            else if constexpr (V == 2)
-                *(uint32_t *)u = *(const uint32_t *)p;
-            else
-                u[0] = p[0];
+            __builtin_memcpy(u, &r, sizeof r);
 #pragma unroll
             for (int i = 0; i < V; i++)
                 v[i] = from<DT>(u[i]);
         }
     }
+    __device__ __forceinline__ void get(const void *base, long at)
+    {
+        set(*(const raw *)((const char *)base + size * at));
+    }
+    /* Past the caches: the next kernel's reads of the input would otherwise
+     * wait for these lines to be written back. */
     __device__ __forceinline__ void put(void *base, long at) const
     {
-        if constexpr (DT == DT_F32) {
-            float *p = (float *)base + at;
+        raw r;
 
-            if constexpr (V == 4)
-                *(f32x4 *)p = *(const f32x4 *)v;
-            else if constexpr (V == 2)
-                *(float2 *)p = *(const float2 *)v;
-            else
-                p[0] = v[0];
-        }
+        if constexpr (DT == DT_F32)
+            __builtin_memcpy(&r, v, sizeof r);
         else {
-            uint16_t *p = (uint16_t *)base + at;
             uint16_t u[V];
 
 #pragma unroll
             for (int i = 0; i < V; i++)
                 u[i] = DT == DT_BF16 ? f2bf(v[i]) : __builtin_bit_cast(uint16_t, (_Float16)v[i]);
-            if constexpr (V == 8)
-                *(u32x4 *)p = *(const u32x4 *)u;
-            else if constexpr (V == 4)
-                *(u32x2 *)p = *(const u32x2 *)u;
-            else if constexpr (V == 2)
-                *(uint32_t *)p = *(const uint32_t *)u;
-            else
-                p[0] = u[0];
+            __builtin_memcpy(&r, u, sizeof r);
         }
+        __builtin_nontemporal_store(r, (raw *)((char *)base + size * at));
     }
 };
 
-__device__ __forceinline__ float act_gn(float v, int act)
+template <int ACT> __device__ __forceinline__ float act_gn(float v)
 {
-    if (act == ACT_SILU_K)
+    if (ACT == ACT_SILU_K)
         return v / (1.0f + __expf(-v));
     /* Not fmaxf: a NaN stays one. */
-    if (act == ACT_RELU_K)
+    if (ACT == ACT_RELU_K)
         return v < 0.0f ? 0.0f : v;
-    return act_k(v, act);
+    return act_k(v, ACT);
+}
+
+template <int A> struct act_of {
+    static constexpr int value = A;
+};
+
+/* f called with the activation as a type, outside its loops. */
+template <typename F> __device__ __forceinline__ void with_act(int act, F f)
+{
+    if (act == ACT_RELU_K)
+        f(act_of<ACT_RELU_K>{});
+    else if (act == ACT_GELU_K)
+        f(act_of<ACT_GELU_K>{});
+    else if (act == ACT_SILU_K)
+        f(act_of<ACT_SILU_K>{});
+    else
+        f(act_of<ACT_NONE_K>{});
 }
 
 /* Mean (in two floats) and 1 / sqrt(var + eps) of n values with sum s.x and
@@ -110,50 +136,82 @@ __device__ __forceinline__ struct stat stat_of(double2 s, double n, float eps)
     return r;
 }
 
-/* One workgroup of 1024 per (group, batch): sums, then the same elements again
- * (from L2, or held in registers up to NR vectors per thread). */
-template <int DT, int V>
-__global__ __launch_bounds__(1024) void k_gn_group(const struct groupnorm_desc d)
-{
-    constexpr int NR = 32 / V;
-    __shared__ double2 red[16];
-    const int t = threadIdx.x, grp = blockIdx.x, b = blockIdx.y;
-    const int cg = d.C / d.groups, gv = cg / V;
-    const long n = d.rows * gv;
-    const long xb = d.xo + b * d.xs0 + grp * cg, yb = d.yo + b * d.ys0 + grp * cg;
-    double2 s = {0.0, 0.0};
-    vec<DT, V> keep[NR];
-    const bool held = n <= 1024L * NR;
+/* Vector t, t + T, ... of a group's rows, gv vectors each. */
+template <int T> struct walk {
+    long row;
+    int col, drow, dcol, gv;
 
-    if (held) {
-#pragma unroll
-        for (int k = 0; k < NR; k++) {
-            const long i = t + 1024L * k;
-
-            if (i < n) {
-                keep[k].get(d.X, xb + i / gv * d.xld + i % gv * V);
-#pragma unroll
-                for (int e = 0; e < V; e++) {
-                    const double x = keep[k].v[e];
-
-                    s.x += x;
-                    s.y = fma(x, x, s.y);
-                }
-            }
+    __device__ __forceinline__ walk(unsigned t, unsigned vectors) : gv(vectors)
+    {
+        row = t / vectors;
+        col = t % vectors;
+        drow = T / vectors;
+        dcol = T % vectors;
+    }
+    __device__ __forceinline__ void next()
+    {
+        row += drow;
+        col += dcol;
+        if (col >= gv) {
+            col -= gv;
+            row++;
         }
     }
+};
+
+/* One workgroup of T per (group, batch): sums, then the same elements again:
+ * up to NR vectors per thread, held in registers with their g and b (which are
+ * read while the sums are added up), or from the caches (NR = 0). */
+template <int DT, int V, int T, int NR>
+__global__ __launch_bounds__(T) void k_gn_group(const struct groupnorm_desc d)
+{
+    __shared__ double2 red[T / 64];
+    const int t = threadIdx.x, grp = blockIdx.x, b = blockIdx.y;
+    const int cg = d.C / d.groups, gv = cg / V;
+    const long xb = d.xo + b * d.xs0 + (long)grp * cg, yb = d.yo + b * d.ys0 + (long)grp * cg;
+    double2 s = {0.0, 0.0};
+    vec<DT, V> keep[NR + 1];
+    float ga[NR + 1][V], be[NR + 1][V];
+    auto add = [&](const vec<DT, V> &x) {
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+            const double xe = x.v[e];
+
+            s.x += xe;
+            s.y = fma(xe, xe, s.y);
+        }
+    };
+    auto affine = [&](int col, float *g, float *be) {
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+            g[e] = d.g ? d.g[grp * cg + col * V + e] : 1.0f;
+            be[e] = d.b ? d.b[grp * cg + col * V + e] : 0.0f;
+        }
+    };
+    walk<T> at(t, gv);
+
+    if constexpr (NR > 0) {
+#pragma unroll
+        for (int k = 0; k < NR; k++, at.next())
+            if (at.row < d.rows)
+                keep[k].get(d.X, xb + at.row * d.xld + at.col * V);
+        at = walk<T>(t, gv);
+#pragma unroll
+        for (int k = 0; k < NR; k++, at.next())
+            if (at.row < d.rows)
+                affine(at.col, ga[k], be[k]);
+        at = walk<T>(t, gv);
+#pragma unroll
+        for (int k = 0; k < NR; k++, at.next())
+            if (at.row < d.rows)
+                add(keep[k]);
+    }
     else
-        for (long i = t; i < n; i += 1024) {
+        for (; at.row < d.rows; at.next()) {
             vec<DT, V> x;
 
-            x.get(d.X, xb + i / gv * d.xld + i % gv * V);
-#pragma unroll
-            for (int e = 0; e < V; e++) {
-                const double xe = x.v[e];
-
-                s.x += xe;
-                s.y = fma(xe, xe, s.y);
-            }
+            x.get(d.X, xb + at.row * d.xld + at.col * V);
+            add(x);
         }
     for (int o = 32; o > 0; o >>= 1) {
         s.x += __shfl_xor(s.x, o, 64);
@@ -163,81 +221,114 @@ __global__ __launch_bounds__(1024) void k_gn_group(const struct groupnorm_desc d
         red[t >> 6] = s;
     __syncthreads();
     s = red[0];
-    for (int i = 1; i < 16; i++) {
+    for (int i = 1; i < T / 64; i++) {
         s.x += red[i].x;
         s.y += red[i].y;
     }
     const struct stat st = stat_of(s, (double)d.rows * cg, d.eps);
-    auto apply = [&](vec<DT, V> &x, long i) {
-        const int c = (int)(i % gv) * V;
 
+    with_act(d.act, [&](auto act) {
+        auto apply = [&](vec<DT, V> &x, const float *g, const float *be) {
 #pragma unroll
-        for (int e = 0; e < V; e++) {
-            const float g = d.g ? d.g[grp * cg + c + e] : 1.0f;
-            const float be = d.b ? d.b[grp * cg + c + e] : 0.0f;
+            for (int e = 0; e < V; e++)
+                x.v[e] = act_gn<decltype(act)::value>(
+                    fmaf((x.v[e] - st.hi) - st.lo, st.rs * g[e], be[e]));
+            x.put(d.Y, yb + at.row * d.yld + at.col * V);
+        };
 
-            x.v[e] = act_gn(fmaf((x.v[e] - st.hi) - st.lo, st.rs * g, be), d.act);
-        }
-        x.put(d.Y, yb + i / gv * d.yld + c);
-    };
-
-    if (held) {
+        at = walk<T>(t, gv);
+        if constexpr (NR > 0) {
 #pragma unroll
-        for (int k = 0; k < NR; k++) {
-            const long i = t + 1024L * k;
-
-            if (i < n)
-                apply(keep[k], i);
+            for (int k = 0; k < NR; k++, at.next())
+                if (at.row < d.rows)
+                    apply(keep[k], ga[k], be[k]);
         }
-    }
-    else
-        for (long i = t; i < n; i += 1024) {
-            vec<DT, V> x;
+        else
+            for (; at.row < d.rows; at.next()) {
+                vec<DT, V> x;
 
-            x.get(d.X, xb + i / gv * d.xld + i % gv * V);
-            apply(x, i);
-        }
+                x.get(d.X, xb + at.row * d.xld + at.col * V);
+                affine(at.col, ga[0], be[0]);
+                apply(x, ga[0], be[0]);
+            }
+    });
 }
 
-/* Rows of chunk blockIdx.x of batch blockIdx.y. */
+/* This workgroup's rows of batch entry blockIdx.y. */
 __device__ __forceinline__ void chunk_rows(const struct groupnorm_desc &d, long *r0, long *r1)
 {
-    const long per = (d.rows + d.chunks - 1) / d.chunks;
+    const long per = (d.rows + gridDim.x - 1) / gridDim.x;
 
     *r0 = min(d.rows, blockIdx.x * per);
     *r1 = min(d.rows, *r0 + per);
 }
 
+/* n vectors, `step` elements apart from element `at` of p, of which the next
+ * AHEAD are under way. */
+template <int DT, int V, int AHEAD> struct stream {
+    typedef typename vec<DT, V>::raw raw;
+    const char *p;
+    long step, n;
+    raw x[AHEAD];
+
+    __device__ __forceinline__ raw load(long k) const
+    {
+        return *(const raw *)(p + min(k, n - 1) * step);
+    }
+    __device__ __forceinline__ void start(const void *base, long at, long step_, long n_)
+    {
+        p = (const char *)base + vec<DT, V>::size * at;
+        step = vec<DT, V>::size * step_;
+        n = n_;
+        if (n > 0)
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++)
+                x[i] = load(i);
+    }
+    /* f on each, with its number. */
+    template <typename F> __device__ __forceinline__ void run(F f)
+    {
+        for (long k = 0; k < n; k += AHEAD)
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++)
+                if (k + i < n) {
+                    vec<DT, V> v;
+
+                    v.set(x[i]);
+                    if (k + i + AHEAD < n)
+                        x[i] = load(k + i + AHEAD);
+                    f(v, k + i);
+                }
+    }
+};
+
 /* Sums of a chunk of rows, per group. A thread keeps one column of V channels
- * (or, where a row has more than 256 of them, one of each block of 256) and
- * walks every (256 / columns)-th row; a group's threads are then added in
+ * (or, where a row has more than TH of them, one of each block of TH) and
+ * walks every (TH / columns)-th row; a group's threads are then added in
  * order. */
 template <int DT, int V>
-__global__ __launch_bounds__(256) void k_gn_stats(const struct groupnorm_desc d)
+__global__ __launch_bounds__(TH) void k_gn_stats(const struct groupnorm_desc d)
 {
-    __shared__ double2 red[256];
+    __shared__ double2 red[TH];
     const int t = threadIdx.x, b = blockIdx.y;
     const int cv = d.C / V, gv = d.C / d.groups / V;
-    double2 *const part = (double2 *)d.part + ((long)b * d.chunks + blockIdx.x) * d.groups;
+    double2 *const part = (double2 *)d.part + (long)b * d.groups * d.chunks + blockIdx.x;
     long r0, r1;
 
     chunk_rows(d, &r0, &r1);
-    const int w = min(cv, 256), lanes = 256 / w;
+    const int w = min(cv, TH), lanes = TH / w;
     const int col = t % w, row = t / w;
 
-    /* Groups that reach over two blocks of columns add to what is there. */
-    for (int g = t; g < d.groups; g += 256)
-        part[g] = double2{0.0, 0.0};
     for (int c0 = 0; c0 < cv; c0 += w) {
         double2 s = {0.0, 0.0};
         const int c = c0 + col;
 
-        if (c < cv && row < lanes)
-#pragma unroll 4
-            for (long r = r0 + row; r < r1; r += lanes) {
-                vec<DT, V> x;
+        if (c < cv && row < lanes) {
+            stream<DT, V, AHEAD_SUMS> in;
 
-                x.get(d.X, d.xo + b * d.xs0 + r * d.xld + (long)c * V);
+            in.start(d.X, d.xo + b * d.xs0 + (r0 + row) * d.xld + (long)c * V,
+                     (long)lanes * d.xld, (r1 - r0 - row + lanes - 1) / lanes);
+            in.run([&](vec<DT, V> &x, long) {
 #pragma unroll
                 for (int e = 0; e < V; e++) {
                     const double xe = x.v[e];
@@ -245,59 +336,108 @@ __global__ __launch_bounds__(256) void k_gn_stats(const struct groupnorm_desc d)
                     s.x += xe;
                     s.y = fma(xe, xe, s.y);
                 }
-            }
+            });
+        }
         __syncthreads();
         red[t] = s;
         __syncthreads();
+        /* The threads of a group (columns a to e of every row), by 16 lanes. */
         const int g0 = c0 / gv, g1 = (min(c0 + w, cv) - 1) / gv;
 
-        for (int g = g0 + t; g <= g1; g += 256) {
-            double2 q = part[g];
+        for (int g = g0 + t / 16; g <= g1; g += TH / 16) {
             const int a = max(c0, g * gv) - c0, e = min(min(c0 + w, cv), (g + 1) * gv) - c0;
+            double2 q = {0.0, 0.0};
 
-            for (int k = 0; k < lanes; k++)
-                for (int i = a; i < e; i++) {
-                    q.x += red[k * w + i].x;
-                    q.y += red[k * w + i].y;
+            for (int j = t % 16, k = j / (e - a), i = j % (e - a); k < lanes;) {
+                q.x += red[k * w + a + i].x;
+                q.y += red[k * w + a + i].y;
+                i += 16;
+                while (i >= e - a) {
+                    i -= e - a;
+                    k++;
                 }
-            part[g] = q;
+            }
+            for (int o = 8; o > 0; o >>= 1) {
+                q.x += __shfl_xor(q.x, o, 16);
+                q.y += __shfl_xor(q.y, o, 16);
+            }
+            if (t % 16 == 0) {
+                /* Groups that reach over two blocks of columns add to what is
+                 * there. */
+                if (c0 > g * gv) {
+                    q.x += part[(long)g * d.chunks].x;
+                    q.y += part[(long)g * d.chunks].y;
+                }
+                part[(long)g * d.chunks] = q;
+            }
         }
     }
 }
 
-/* The chunk's rows normalised: mean and deviation of each group from the
- * sums of all chunks, in order. */
+/* A group's sums over all chunks, in order, by a wave. */
+__device__ __forceinline__ struct stat group_stat(const struct groupnorm_desc &d, int b, int g)
+{
+    const double2 *const p = (const double2 *)d.part + ((long)b * d.groups + g) * d.chunks;
+    double2 s = {0.0, 0.0};
+
+    for (int k = threadIdx.x & 63; k < d.chunks; k += 64) {
+        const double2 x = p[k];
+
+        s.x += x.x;
+        s.y += x.y;
+    }
+    for (int o = 32; o > 0; o >>= 1) {
+        s.x += __shfl_xor(s.x, o, 64);
+        s.y += __shfl_xor(s.y, o, 64);
+    }
+    return stat_of(s, (double)d.rows * (d.C / d.groups), d.eps);
+}
+
+/* Where there are many sums, they are added up once. */
+__global__ __launch_bounds__(256) void k_gn_sums(const struct groupnorm_desc d)
+{
+    const int g = blockIdx.x * 4 + (threadIdx.x >> 6), b = blockIdx.y;
+
+    if (g >= d.groups)
+        return;
+    const struct stat s = group_stat(d, b, g);
+
+    if ((threadIdx.x & 63) == 0)
+        ((struct stat *)d.stats)[b * d.groups + g] = s;
+}
+
+/* The chunk's rows normalised by mean and deviation of each group. */
 template <int DT, int V>
-__global__ __launch_bounds__(256) void k_gn_apply(const struct groupnorm_desc d)
+__global__ __launch_bounds__(TH) void k_gn_apply(const struct groupnorm_desc d)
 {
     extern __shared__ struct stat st[];
     const int t = threadIdx.x, b = blockIdx.y;
-    const int cg = d.C / d.groups, cv = d.C / V, gv = cg / V;
-    const double2 *const part = (const double2 *)d.part + (long)b * d.chunks * d.groups;
+    const int cv = d.C / V, gv = d.C / d.groups / V;
     long r0, r1;
 
     chunk_rows(d, &r0, &r1);
-    for (int g = t >> 6; g < d.groups; g += 4) {
-        double2 s = {0.0, 0.0};
-
-        for (int k = t & 63; k < d.chunks; k += 64) {
-            const double2 x = part[(long)k * d.groups + g];
-
-            s.x += x.x;
-            s.y += x.y;
-        }
-        for (int o = 32; o > 0; o >>= 1) {
-            s.x += __shfl_xor(s.x, o, 64);
-            s.y += __shfl_xor(s.y, o, 64);
-        }
-        if ((t & 63) == 0)
-            st[g] = stat_of(s, (double)d.rows * cg, d.eps);
-    }
-    __syncthreads();
-    const int w = min(cv, 256), lanes = 256 / w;
+    const int w = min(cv, TH), lanes = TH / w;
     const int col = t % w, row = t / w;
+    const long n = row < lanes ? (r1 - r0 - row + lanes - 1) / lanes : 0;
+    stream<DT, V, AHEAD_APPLY> in;
 
-    for (int c = col; c < cv && row < lanes; c += w) {
+    /* The first rows, on their way during the sums. */
+    in.start(d.X, d.xo + b * d.xs0 + (r0 + row) * d.xld + (long)col * V, (long)lanes * d.xld, n);
+    if (d.stats)
+        for (int g = t; g < d.groups; g += TH)
+            st[g] = ((const struct stat *)d.stats)[b * d.groups + g];
+    else
+        for (int g = t >> 6; g < d.groups; g += TH / 64) {
+            const struct stat q = group_stat(d, b, g);
+
+            if ((t & 63) == 0)
+                st[g] = q;
+        }
+    __syncthreads();
+    for (int c = col; c < cv && n > 0; c += w) {
+        if (c != col)
+            in.start(d.X, d.xo + b * d.xs0 + (r0 + row) * d.xld + (long)c * V,
+                     (long)lanes * d.xld, n);
         const struct stat q = st[c / gv];
         float a[V], be[V];
 
@@ -306,37 +446,40 @@ __global__ __launch_bounds__(256) void k_gn_apply(const struct groupnorm_desc d)
             a[e] = q.rs * (d.g ? d.g[c * V + e] : 1.0f);
             be[e] = d.b ? d.b[c * V + e] : 0.0f;
         }
-#pragma unroll 4
-        for (long r = r0 + row; r < r1; r += lanes) {
-            vec<DT, V> x;
+        with_act(d.act, [&](auto act) {
+            char *y = (char *)d.Y + vec<DT, V>::size *
+                                        (d.yo + b * d.ys0 + (r0 + row) * d.yld + (long)c * V);
+            const long ystep = (long)lanes * d.yld;
 
-            x.get(d.X, d.xo + b * d.xs0 + r * d.xld + (long)c * V);
+            in.run([&](vec<DT, V> &x, long k) {
 #pragma unroll
-            for (int e = 0; e < V; e++)
-                x.v[e] = act_gn(fmaf((x.v[e] - q.hi) - q.lo, a[e], be[e]), d.act);
-            x.put(d.Y, d.yo + b * d.ys0 + r * d.yld + (long)c * V);
-        }
+                for (int e = 0; e < V; e++)
+                    x.v[e] = act_gn<decltype(act)::value>(
+                        fmaf((x.v[e] - q.hi) - q.lo, a[e], be[e]));
+                x.put(y, k * ystep);
+            });
+        });
     }
 }
 
 /* ------------------------------------------------------------ launch */
 
-/* Row chunks per batch entry, or 1: one workgroup per group then holds its
- * elements (32 per thread) or the whole is small. */
+/* Row chunks per batch entry, or 1: one workgroup per group. */
 static void plan(struct groupnorm_desc *d)
 {
     const long elems = d->rows * (d->C / d->groups);
     const int cu = dev_cu_count();
     long chunks = 1;
 
-    if (elems > 32 * 1024) {
-        chunks = (4L * cu + d->nb - 1) / d->nb;
-        if (chunks > d->rows / 8)
-            chunks = d->rows / 8;
-        if (chunks > 1024)
-            chunks = 1024;
-        if (chunks < 1)
-            chunks = 1;
+    if (elems > (d->C / d->groups * (d->dt == DT_F32 ? 4 : 2) < 16 ? SPLIT_ABOVE_NARROW : SPLIT_ABOVE)) {
+        chunks = (2L * cu + d->nb - 1) / d->nb;
+        /* Two vectors of eight per thread. */
+        if (chunks > d->rows * d->C / (16 * TH))
+            chunks = d->rows * d->C / (16 * TH);
+        if (chunks > d->rows)
+            chunks = d->rows;
+        if (chunks < 2)
+            chunks = 2;
     }
     d->chunks = (int)chunks;
 }
@@ -344,18 +487,34 @@ static void plan(struct groupnorm_desc *d)
 extern "C" size_t groupnorm_ws_bytes(struct groupnorm_desc *d)
 {
     plan(d);
-    return d->chunks > 1 ? 16 * (size_t)d->nb * d->chunks * d->groups : 0;
+    return d->chunks > 1
+               ? (size_t)d->nb * d->groups * (16 * (size_t)d->chunks + sizeof(struct stat))
+               : 0;
 }
 
 template <int DT, int V> static int run(const struct groupnorm_desc *d, hipStream_t s)
 {
-    if (d->chunks == 1)
-        hipLaunchKernelGGL((k_gn_group<DT, V>), dim3(d->groups, d->nb), dim3(1024), 0, s, *d);
+    const dim3 grid(d->groups, d->nb);
+    int err;
+
+    if (d->chunks == 1) {
+        if (d->rows * (d->C / d->groups) <= 256 * 4)
+            hipLaunchKernelGGL((k_gn_group<DT, V, 256, 16 / V>), grid, dim3(256), 0, s, *d);
+        else if (d->rows * (d->C / d->groups) <= 1024 * 16)
+            hipLaunchKernelGGL((k_gn_group<DT, V, 1024, 16 / V>), grid, dim3(1024), 0, s, *d);
+        else
+            hipLaunchKernelGGL((k_gn_group<DT, V, 1024, 0>), grid, dim3(1024), 0, s, *d);
+    }
     else {
-        hipLaunchKernelGGL((k_gn_stats<DT, V>), dim3(d->chunks, d->nb), dim3(256), 0, s, *d);
-        if (hipGetLastError() != hipSuccess)
-            return hipErrorLaunchFailure;
-        hipLaunchKernelGGL((k_gn_apply<DT, V>), dim3(d->chunks, d->nb), dim3(256),
+        hipLaunchKernelGGL((k_gn_stats<DT, V>), dim3(d->chunks, d->nb), dim3(TH), 0, s, *d);
+        err = hipGetLastError();
+        if (err == hipSuccess && d->stats) {
+            hipLaunchKernelGGL(k_gn_sums, dim3((d->groups + 3) / 4, d->nb), dim3(256), 0, s, *d);
+            err = hipGetLastError();
+        }
+        if (err != hipSuccess)
+            return err;
+        hipLaunchKernelGGL((k_gn_apply<DT, V>), dim3((d->chunks + 1) / 2, d->nb), dim3(TH),
                            d->groups * sizeof(struct stat), s, *d);
     }
     return hipGetLastError();
@@ -378,6 +537,11 @@ extern "C" int launch_groupnorm(struct groupnorm_desc *d, void *ws, size_t ws_by
     if (need && (!ws || ws_bytes < need))
         d->chunks = 1;
     d->part = (float *)ws;
+    /* A launch of its own for the sums where every workgroup would read more
+     * than 128 KiB of them. */
+    d->stats = d->chunks > 1 && (long)d->chunks * d->groups > 8192
+                   ? (char *)ws + 16 * (size_t)d->nb * d->groups * d->chunks
+                   : NULL;
     return d->dt == DT_F32   ? run_dt<DT_F32>(d, (hipStream_t)stream)
            : d->dt == DT_F16 ? run_dt<DT_F16>(d, (hipStream_t)stream)
                              : run_dt<DT_BF16>(d, (hipStream_t)stream);

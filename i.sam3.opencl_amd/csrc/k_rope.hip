@@ -6,6 +6,19 @@
  */
 #include "k_common.h"
 
+/* Workgroups per compute unit beyond which a thread takes more rows (tables) or
+ * heads, and heads whose loads are under way together. us with 2 / 4 / 8 heads:
+ * 32774 rows of 8 x 128 halves 36.4 / 33.8 / 32.3; a table of 131072 x 64 pairs
+ * the same within 3 % from 8 to 32 workgroups. */
+#define TABLE_WG 16
+#define ROWS_WG 8L
+#define HEADS_AHEAD 4
+
+/* Results go past the caches: written through them, the lines are held until
+ * the kernel's end and go out then. The rows above take 23.2 us (139 MB, 6.0
+ * TB/s) for 33.8, the table 13.3 (67 MB) for 14.2. */
+#define STORE(p, x) __builtin_nontemporal_store(x, p)
+
 /* ------------------------------------------------------------ tables */
 
 /* cos and sin of a turn's fraction. Whole turns and quarters come off in 64
@@ -35,30 +48,55 @@ __device__ __forceinline__ float2 cos_sin_turns(double t)
     return float2{(q + 1) & 2 ? -a : a, q & 2 ? -b : b};
 }
 
-/* A thread per angle, pairs fastest: consecutive lanes write consecutive
- * (cos, sin). */
-__global__ __launch_bounds__(256) void k_rope_table(const struct rope_table_desc d)
+/* A thread keeps one pair (or two where their number is even, so that it
+ * writes 16 bytes) and walks rows blockIdx.y step apart. */
+template <int N> __global__ __launch_bounds__(256) void k_rope_table(const struct rope_table_desc d)
 {
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    const int units = d.pairs / N, per = 256 / min(units, 256);
+    const int t = threadIdx.x, u = blockIdx.x * 256 + t % min(units, 256);
 
-    if (i >= (long)d.npos * d.pairs)
+    if (u >= units || t / min(units, 256) >= per)
         return;
-    const int p = (int)(i / d.pairs), j = (int)(i % d.pairs);
-    int pos = d.pos ? d.pos[p] : p;
+    double f[N];
 
-    if (d.W)
-        pos = j < d.pairs / 2 ? pos % d.W : pos / d.W;
-    const float2 cs = cos_sin_turns(pos * d.turns[j]);
+#pragma unroll
+    for (int e = 0; e < N; e++)
+        f[e] = d.turns[u * N + e];
+    for (int p = blockIdx.y * per + t / min(units, 256); p < d.npos; p += gridDim.y * per) {
+        const int pos = d.pos ? d.pos[p] : p;
+        float v[2 * N];
 
-    ((float2 *)d.table)[i] = float2{cs.x * d.mul, cs.y * d.mul};
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+            const int at = !d.W ? pos : u * N + e < d.pairs / 2 ? pos % d.W : pos / d.W;
+            const float2 cs = cos_sin_turns(at * f[e]);
+
+            v[2 * e] = cs.x * d.mul;
+            v[2 * e + 1] = cs.y * d.mul;
+        }
+        float *const o = d.table + 2 * ((long)p * d.pairs + u * N);
+
+        if constexpr (N == 2)
+            STORE((f32x4 *)o, (f32x4{v[0], v[1], v[2], v[3]}));
+        else
+            *(float2 *)o = float2{v[0], v[1]};
+    }
 }
 
 extern "C" int launch_rope_table(const struct rope_table_desc *d, void *stream)
 {
-    const long n = (long)d->npos * d->pairs;
+    const int n = d->pairs % 2 == 0 && (uintptr_t)d->table % 16 == 0 ? 2 : 1;
+    const int units = d->pairs / n, per = 256 / (units < 256 ? units : 256);
+    long y = ((long)d->npos + per - 1) / per;
 
-    hipLaunchKernelGGL(k_rope_table, dim3((unsigned)((n + 255) / 256)), dim3(256), 0,
-                       (hipStream_t)stream, *d);
+    if (y > TABLE_WG * dev_cu_count())
+        y = TABLE_WG * dev_cu_count();
+    const dim3 grid((unsigned)((units + 255) / 256), (unsigned)y);
+
+    if (n == 2)
+        hipLaunchKernelGGL(k_rope_table<2>, grid, dim3(256), 0, (hipStream_t)stream, *d);
+    else
+        hipLaunchKernelGGL(k_rope_table<1>, grid, dim3(256), 0, (hipStream_t)stream, *d);
     return hipGetLastError();
 }
 
@@ -102,7 +140,7 @@ template <int DT, int N> __device__ __forceinline__ void put(char *p, const floa
 {
     if constexpr (DT == DT_F32) {
         if constexpr (N == 4)
-            *(f32x4 *)p = *(const f32x4 *)v;
+            STORE((f32x4 *)p, *(const f32x4 *)v);
         else
             for (int i = 0; i < N; i++)
                 ((float *)p)[i] = v[i];
@@ -114,7 +152,7 @@ template <int DT, int N> __device__ __forceinline__ void put(char *p, const floa
         for (int i = 0; i < N; i++)
             u[i] = to<DT>(v[i]);
         if constexpr (N == 8)
-            *(u32x4 *)p = *(const u32x4 *)u;
+            STORE((u32x4 *)p, *(const u32x4 *)u);
         else
             for (int i = 0; i < N; i++)
                 ((uint16_t *)p)[i] = u[i];
@@ -178,32 +216,43 @@ __global__ __launch_bounds__(256) void k_rope_rows(const struct rope_rows_desc d
         if (!d.copy)
             return;
     }
-#pragma unroll 4
-    for (int h = blockIdx.y; h < d.heads; h += gridDim.y) {
-        float v[2 * P], o[2 * P];
-        const char *xh = x + S * (h * d.xs1);
-        char *yh = y + S * (h * d.ys1);
+    for (int h0 = blockIdx.y; h0 < d.heads; h0 += HEADS_AHEAD * gridDim.y) {
+        float v[HEADS_AHEAD][2 * P];
 
-        if (HALVES) {
-            get<DT, N>(xh + S * c0, v);
-            get<DT, N>(xh + S * c1, v + N);
-        }
-        else
-            get<DT, M>(xh + S * c0, v);
 #pragma unroll
-        for (int k = 0; k < P; k++) {
-            const int ia = HALVES ? k : 2 * k, ib = HALVES ? N + k : 2 * k + 1;
-            const float c = cs[2 * k], s = cs[2 * k + 1];
+        for (int j = 0; j < HEADS_AHEAD; j++) {
+            const char *xh = x + S * (min(h0 + j * (int)gridDim.y, d.heads - 1) * d.xs1);
 
-            o[ia] = turn ? fmaf(v[ia], c, -(v[ib] * s)) : v[ia];
-            o[ib] = turn ? fmaf(v[ia], s, v[ib] * c) : v[ib];
+            if (HALVES) {
+                get<DT, N>(xh + S * c0, v[j]);
+                get<DT, N>(xh + S * c1, v[j] + N);
+            }
+            else
+                get<DT, M>(xh + S * c0, v[j]);
         }
-        if (HALVES) {
-            put<DT, N>(yh + S * c0, o);
-            put<DT, N>(yh + S * c1, o + N);
+#pragma unroll
+        for (int j = 0; j < HEADS_AHEAD; j++) {
+            const int h = h0 + j * gridDim.y;
+            char *yh = y + S * (h * d.ys1);
+            float o[2 * P];
+
+            if (h >= d.heads)
+                break;
+#pragma unroll
+            for (int k = 0; k < P; k++) {
+                const int ia = HALVES ? k : 2 * k, ib = HALVES ? N + k : 2 * k + 1;
+                const float c = cs[2 * k], s = cs[2 * k + 1];
+
+                o[ia] = turn ? fmaf(v[j][ia], c, -(v[j][ib] * s)) : v[j][ia];
+                o[ib] = turn ? fmaf(v[j][ia], s, v[j][ib] * c) : v[j][ib];
+            }
+            if (HALVES) {
+                put<DT, N>(yh + S * c0, o);
+                put<DT, N>(yh + S * c1, o + N);
+            }
+            else
+                put<DT, M>(yh + S * c0, o);
         }
-        else
-            put<DT, M>(yh + S * c0, o);
     }
 }
 
@@ -215,7 +264,7 @@ static int run(const struct rope_rows_desc *d, hipStream_t s)
     const long n = (long)d->nb * d->rows * units;
     const long blocks = (n + 255) / 256;
     /* Heads are spread over workgroups until the device is full. */
-    long hy = (8L * dev_cu_count() + blocks - 1) / blocks;
+    long hy = (ROWS_WG * dev_cu_count() + blocks - 1) / blocks;
 
     if (hy > d->heads)
         hy = d->heads;

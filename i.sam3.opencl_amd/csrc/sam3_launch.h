@@ -410,8 +410,9 @@ struct groupnorm_desc {
     long rows;
     const float *g, *b;
     float eps;
-    int chunks; /* set by groupnorm_ws_bytes / launch_groupnorm */
+    int chunks; /* set by groupnorm_ws_bytes / launch_groupnorm, as what follows */
     float *part;
+    void *stats;
 };
 
 /* Workspace (0: none wanted); with less, or NULL, one workgroup per (batch,
