@@ -124,11 +124,9 @@ __device__ __forceinline__ u32x4 row16(const char *p, int cb, int hdb)
     return v;
 }
 
-/* One 16-byte step of S^T = K Q^T: the K row chunk at kp, Q's likewise. */
-template <int DT> __device__ __forceinline__ f32x16 k_step(const char *kp, u32x4 q, f32x16 s)
+/* One 16-byte step of S^T = K Q^T. */
+template <int DT> __device__ __forceinline__ f32x16 k_step(u32x4 k, u32x4 q, f32x16 s)
 {
-    const u32x4 k = *(const u32x4 *)kp;
-
     if constexpr (DT == DT_F32) {
         const f32x4 kx = __builtin_bit_cast(f32x4, k), qx = __builtin_bit_cast(f32x4, q);
 
@@ -209,6 +207,47 @@ template <int N> __device__ __forceinline__ void copies_and_barrier()
                  :
                  : "n"(N)
                  : "memory");
+}
+
+/* Columns c to c + 31 of an output row: this lane's half (h) of the sums in o,
+ * times inv. */
+template <int DT, bool VEC>
+__device__ __forceinline__ void put_block(char *op, int c, int hd, int h, const f32x16 &o, float inv)
+{
+#pragma unroll
+    for (int q = 0; q < 4; q += 2, c += 16) {
+        float x[8];
+
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            x[e] = o[4 * q + e] * inv;
+        if constexpr (!VEC) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int ce = c + 8 * (e / 4) + 4 * h + e % 4;
+
+                if (ce < hd)
+                    put_elem<DT>(op, ce, x[e]);
+            }
+        }
+        else if constexpr (DT == DT_F32) {
+            if (c + 4 * h < hd)
+                *(f32x4 *)(op + 4 * (c + 4 * h)) = f32x4{x[0], x[1], x[2], x[3]};
+            if (c + 8 + 4 * h < hd)
+                *(f32x4 *)(op + 4 * (c + 8 + 4 * h)) = f32x4{x[4], x[5], x[6], x[7]};
+        }
+        else {
+            /* Lanes 32 apart exchange halves: 8 columns in a row each. */
+            const auto u = __builtin_amdgcn_permlane32_swap(
+                pack2<DT>(x[0], x[1]), pack2<DT>(x[4], x[5]), false, false);
+            const auto v = __builtin_amdgcn_permlane32_swap(
+                pack2<DT>(x[2], x[3]), pack2<DT>(x[6], x[7]), false, false);
+
+            if (c + 8 * h < hd)
+                *(u32x4 *)(op + 2 * (c + 8 * h)) =
+                    u32x4{(uint32_t)u[0], (uint32_t)v[0], (uint32_t)u[1], (uint32_t)v[1]};
+        }
+    }
 }
 
 /* DP: head width padded to 32, 64, 128 or 256. WM waves share the rows of a
@@ -376,15 +415,16 @@ __global__ __launch_bounds__(256, OCC) void k_xattn(const struct xattn_desc a)
         if (half) {
 #pragma unroll
             for (int i = 0; i < CH / 2; i++)
-                s[0] = k_step<DT>(ldk + rk::at(lr) + 16 * ((2 * i + h) ^ rk::swz(lr)), qf[i], s[0]);
+                s[0] = k_step<DT>(*(const u32x4 *)(ldk + rk::at(lr) + 16 * ((2 * i + h) ^ rk::swz(lr))),
+                                  qf[i], s[0]);
         }
         else {
 #pragma unroll
             for (int i = 0; i < CH / 2; i++)
 #pragma unroll
                 for (int n = 0; n < NB; n++)
-                    s[n] = k_step<DT>(ldk + rk::at(n * 32) + rk::at(lr) +
-                                          16 * ((2 * i + h) ^ rk::swz(lr)),
+                    s[n] = k_step<DT>(*(const u32x4 *)(ldk + rk::at(n * 32) + rk::at(lr) +
+                                                       16 * ((2 * i + h) ^ rk::swz(lr))),
                                       qf[i], s[n]);
         }
         if (!ALL && (KW == 64 ? ~keep != 0 : (uint32_t)keep != 0xffffffffu)) {
@@ -607,44 +647,218 @@ __global__ __launch_bounds__(256, OCC) void k_xattn(const struct xattn_desc a)
                                         (long)iq * a.old);
 
 #pragma unroll
-    for (int d = 0; d < DP / 32; d++) {
-        if (d % WK != wk)
-            continue;
+    for (int d = 0; d < DP / 32; d++)
+        if (d % WK == wk)
+            put_block<DT, VEC>(op, 32 * d, a.hd, h, o[d], inv);
+}
+
+/* At most 64 keys (a prompt) and many rows: bound by reading Q and writing O. A
+ * workgroup keeps one unit's K and V and each of its waves walks blocks of 32
+ * rows, the next block's rows of Q under way; all weights of a row are there at
+ * once, so no maximum runs. Fragments of K and V stay in registers where the
+ * types are 16 bits wide. us at batch 8, 5184 rows, 37 keys, 8 heads of 32 and 64
+ * bf16 (43 and 85 MB): 12.3 and 21.2 (3.5 and 4.0 TB/s), 13.5 and 24.7 with a
+ * lane per row of Q and O in memory, 16.6 and 24.6 by k_xattn; 13.4 for the first
+ * with O through the caches, 14.7 with two blocks ahead, 17.1 with 8 instead of 4
+ * workgroups per compute unit. Floats, 20 keys, heads of 32: 25.2, 30.2 by
+ * k_xattn. */
+template <int DT, int DP, int NB>
+__global__ __launch_bounds__(256, 2) void k_xattn_few(const struct xattn_desc a)
+{
+    constexpr int S = xt<DT>::size;
+    constexpr int RB = DP * S, CH = RB / 16;
+    typedef row_k<RB> rk;
+    typedef row_v<RB, DT> rv;
+    constexpr int NK = NB * 32 / rk::RPK;               /* copies for K or V, 1 KiB each */
+    constexpr int KT = NK * (1024 + rk::PAD);
+    constexpr int NV = DT == DT_F32 ? 0 : 2 * NB * (DP / 32);
+    constexpr int QP = RB + 16;                         /* pitch of a wave's own rows */
+    constexpr int KV = KT + NK * (1024 + rv::PAD);
+    __shared__ __attribute__((aligned(1024))) char lds[KV + 4 * 32 * QP];
+    const int tid = threadIdx.x, l = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int h = l >> 5, lr = l & 31;
+    char *const own = lds + KV + w * 32 * QP;
+    const unsigned item = (blockIdx.x & 7) * ((a.items + 7) / 8) + (blockIdx.x >> 3);
+
+    if (item >= (unsigned)a.items)
+        return;
+    const unsigned part = item / a.units, unit = item - part * a.units;
+    const int b = unit / (unsigned)a.kvh, kh = unit - b * a.kvh;
+    const int nq = a.qlen ? max(0, min(a.qlen[b], a.Nq)) : a.Nq;
+    const int nk = a.klen ? max(0, min(a.klen[b], a.Nk)) : a.Nk;
+    const int rows = a.grp * nq, blocks = (rows + 31) / 32, hdb = a.hd * S;
+    /* This wave's blocks: part, part + parts, ... of four waves each. */
+    const int step = 4 * a.tiles;
+    int blk = 4 * part + w;
+
+    if (4 * (int)part >= blocks)
+        return;
+    /* Rows of Q and O pass through LDS of the wave's own: in memory CH lanes take
+     * a whole row (a lane of each row at a time would be 64 requests). Access i
+     * of lane l: row i 64 / CH + l / CH, 16 bytes l % CH. */
+    auto row_at = [&](int blk, int i, long off, long s0, long s1, int ld) {
+        const int r = min(blk * 32 + i * (64 / CH) + l / CH, rows - 1);
+        const int hq = a.grp == 1 ? 0 : r / nq, iq = r - hq * nq;
+
+        return S * (off + (long)b * s0 + (long)(kh * a.grp + hq) * s1 + (long)iq * ld) +
+               16 * (l % CH);
+    };
+    u32x4 q[CH / 2];
+    auto load_q = [&](int blk) {
 #pragma unroll
-        for (int q = 0; q < 4; q += 2) {
-            float x[8];
+        for (int i = 0; i < CH / 2; i++)
+            q[i] = 16 * (l % CH) < hdb
+                       ? *(const u32x4 *)((const char *)a.Q + row_at(min(blk, blocks - 1), i, a.qo,
+                                                                     a.qs0, a.qs1, a.qld))
+                       : u32x4{0, 0, 0, 0};
+    };
+    /* K and V: rows past the last key read the last one, columns past hd zeros. */
+    const unsigned lbase = (unsigned)(uintptr_t)lds;
+
+    if (nk > 0) {
+        const int lrow = l / CH;
+        const int ck = 16 * ((l % CH) ^ rk::swz(lrow)), cv = 16 * ((l % CH) ^ rv::swz(lrow));
+        const char *const kb =
+            (const char *)a.K + S * (a.ko + (long)b * a.ks0 + (long)kh * a.ks1);
+        const char *const vb =
+            (const char *)a.V + S * (a.vo + (long)b * a.vs0 + (long)kh * a.vs1);
+
+        for (int c = w; c < NK; c += 4) {
+            const long r = min(c * rk::RPK + lrow, nk - 1);
+
+            g2lds16_at(ck < hdb ? kb + r * a.kld * S + ck : (const char *)&xattn_zeros,
+                       __builtin_amdgcn_readfirstlane(lbase + c * (1024 + rk::PAD)));
+            g2lds16_at(cv < hdb ? vb + r * a.vld * S + cv : (const char *)&xattn_zeros,
+                       __builtin_amdgcn_readfirstlane(lbase + KT + c * (1024 + rv::PAD)));
+        }
+    }
+    /* Keys that count, a bit for each. */
+    const bool in = l < NB * 32 && l < nk;
+    const uint64_t keep = __ballot(in && (!a.kmask || a.kmask[(long)b * a.Nk + min(l, nk - 1)]));
+
+    load_q(blk);
+    copies_and_barrier<0>();
+    /* Rows of V that do not count. */
+    for (int c = tid; c < NB * 32 * CH; c += 256)
+        if (!(keep >> (c / CH) & 1))
+            *(u32x4 *)(lds + KT + rv::at(c / CH) + 16 * (c % CH)) = u32x4{0, 0, 0, 0};
+    copies_and_barrier<0>();
+    auto k_frag = [&](int n, int i) {
+        return *(const u32x4 *)(lds + rk::at(n * 32) + rk::at(lr) +
+                                16 * ((2 * i + h) ^ rk::swz(lr)));
+    };
+    auto v_frag = [&](int f) {
+        const int key = f / (DP / 32) * 16, d = f % (DP / 32);
+        const int row = 4 * h + (l & 15) / 4, c0 = 2 * (l >> 4 & 1) + (l >> 1 & 1);
+        const char *vd = lds + KT + rv::at(key) + rv::at(row) + 8 * (l & 1) +
+                         16 * ((4 * d + c0) ^ rv::swz(row));
+        const u32x2 v0 = lds_tr(vd), v1 = lds_tr(vd + rv::at(8));
+
+        return u32x4{v0.x, v0.y, v1.x, v1.y};
+    };
+    u32x4 kf[NB * (CH / 2)], vf[NV + 1];
+
+    if constexpr (DT != DT_F32) {
+#pragma unroll
+        for (int f = 0; f < NB * (CH / 2); f++)
+            kf[f] = k_frag(f % NB, f / NB);
+#pragma unroll
+        for (int f = 0; f < NV; f++)
+            vf[f] = v_frag(f);
+    }
+    for (; blk < blocks; blk += step) {
+        f32x16 s[NB], o[DP / 32];
+        float mx = NEG_INF, sum = 0.0f;
 
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                x[e] = o[d][4 * q + e] * inv;
-            const int c = 32 * d + 8 * q;
-
-            if constexpr (!VEC) {
+        for (int i = 0; i < CH / 2; i++)
+            *(u32x4 *)(own + (i * (64 / CH) + l / CH) * QP + 16 * (l % CH)) = q[i];
+        load_q(blk + step);
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const int ce = c + 8 * (e / 4) + 4 * h + e % 4;
+        for (int n = 0; n < NB; n++)
+            s[n] = f32x16{0};
+#pragma unroll
+        for (int i = 0; i < CH / 2; i++) {
+            const u32x4 qf = *(const u32x4 *)(own + lr * QP + 16 * (2 * i + h));
 
-                    if (ce < a.hd)
-                        put_elem<DT>(op, ce, x[e]);
+#pragma unroll
+            for (int n = 0; n < NB; n++)
+                s[n] = k_step<DT>(DT == DT_F32 ? k_frag(n, i) : kf[i * NB + n], qf, s[n]);
+        }
+        if (NB == 2 ? ~keep != 0 : (uint32_t)keep != 0xffffffffu)
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+                const uint32_t bits = (uint32_t)(keep >> (32 * n)) >> (4 * h);
+
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (!(bits >> (8 * (i / 4) + i % 4) & 1))
+                        s[n][i] = NEG_INF;
+            }
+#pragma unroll
+        for (int n = 0; n < NB; n++)
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                mx = fmaxf(mx, s[n][i]);
+        const f32x2 mh = both_halves(mx);
+
+        mx = fmaxf(mh.x, mh.y) * a.c;
+        mx = mx == NEG_INF ? 0.0f : mx;
+#pragma unroll
+        for (int n = 0; n < NB; n++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], a.c, -mx));
+                sum += s[n][i];
+            }
+        const f32x2 sh = both_halves(sum);
+
+        sum = sh.x + sh.y;
+#pragma unroll
+        for (int d = 0; d < DP / 32; d++)
+            o[d] = f32x16{0};
+        if constexpr (DT == DT_F32) {
+#pragma unroll
+            for (int n = 0; n < NB; n++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const char *vr = lds + KT + rv::at(n * 32 + 8 * (i / 4)) +
+                                     rv::at(i % 4 + 4 * h) + 4 * lr;
+
+#pragma unroll
+                    for (int d = 0; d < DP / 32; d++)
+                        o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(*(const float *)(vr + 128 * d),
+                                                                    s[n][i], o[d], 0, 0, 0);
                 }
-            }
-            else if constexpr (DT == DT_F32) {
-                if (c + 4 * h < a.hd)
-                    *(f32x4 *)(op + 4 * (c + 4 * h)) = f32x4{x[0], x[1], x[2], x[3]};
-                if (c + 8 + 4 * h < a.hd)
-                    *(f32x4 *)(op + 4 * (c + 8 + 4 * h)) = f32x4{x[4], x[5], x[6], x[7]};
-            }
-            else {
-                /* Lanes 32 apart exchange halves: 8 columns in a row each. */
-                const auto u = __builtin_amdgcn_permlane32_swap(
-                    pack2<DT>(x[0], x[1]), pack2<DT>(x[4], x[5]), false, false);
-                const auto v = __builtin_amdgcn_permlane32_swap(
-                    pack2<DT>(x[2], x[3]), pack2<DT>(x[6], x[7]), false, false);
+        }
+        else {
+#pragma unroll
+            for (int k = 0; k < 2 * NB; k++) {
+                u32x4 p;
 
-                if (c + 8 * h < a.hd)
-                    *(u32x4 *)(op + 2 * (c + 8 * h)) =
-                        u32x4{(uint32_t)u[0], (uint32_t)v[0], (uint32_t)u[1], (uint32_t)v[1]};
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    p[i] = pack2<DT>(s[k / 2][8 * (k & 1) + 2 * i],
+                                     s[k / 2][8 * (k & 1) + 2 * i + 1]);
+#pragma unroll
+                for (int d = 0; d < DP / 32; d++)
+                    o[d] = mfma16<DT>(vf[k * (DP / 32) + d], p, o[d]);
             }
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+
+#pragma unroll
+        for (int d = 0; d < DP / 32; d++)
+            put_block<DT, true>(own + lr * QP, 32 * d, DP, h, o[d], inv);
+#pragma unroll
+        for (int i = 0; i < CH / 2; i++) {
+            const int r = i * (64 / CH) + l / CH;
+            const u32x4 v = *(const u32x4 *)(own + r * QP + 16 * (l % CH));
+
+            if (blk * 32 + r < rows && 16 * (l % CH) < hdb)
+                __builtin_nontemporal_store(
+                    v, (u32x4 *)((char *)a.O + row_at(blk, i, a.oo, a.os0, a.os1, a.old)));
         }
     }
 }
@@ -769,6 +983,17 @@ static void plan(struct xattn_desc *d)
     if (wm < least)
         wm = least;
     d->splits = 1;
+    d->few = d->vec && d->hd <= 64 && d->Nk <= 64;
+    if (d->few) {
+        /* Workgroups of a unit, a wave for each block of 32 rows at most. */
+        long parts = 4 * cu / d->units;
+
+        if (parts > (rows + 127) / 128)
+            parts = (rows + 127) / 128;
+        d->tiles = parts < 1 ? 1 : (int)parts;
+        d->items = (long)d->units * d->tiles;
+        return;
+    }
     if (!d->vec)
         wm = rb >= 1024 ? 4 : 2;
     else if (d->Nk > 256) {
@@ -821,9 +1046,21 @@ static int run(const struct xattn_desc *d, hipStream_t s)
     return hipGetLastError();
 }
 
+template <int DT, int DP, int NB> static int run_few(const struct xattn_desc *d, hipStream_t s)
+{
+    const long grid = (d->items + 7) / 8 * 8;
+
+    hipLaunchKernelGGL((k_xattn_few<DT, DP, NB>), dim3((unsigned)grid), dim3(256), 0, s, *d);
+    return hipGetLastError();
+}
+
 template <int DT, int DP> static int run_wm(const struct xattn_desc *d, hipStream_t s)
 {
     constexpr int RB = DP * xt<DT>::size;
+
+    if constexpr (DP <= 64)
+        if (d->few)
+            return d->Nk <= 32 ? run_few<DT, DP, 1>(d, s) : run_few<DT, DP, 2>(d, s);
 
     if (!d->vec) {
         if constexpr (RB == 1024)

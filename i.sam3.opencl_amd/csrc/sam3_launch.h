@@ -358,7 +358,7 @@ struct xattn_desc {
     const unsigned char *kmask;
     int units, kvh, grp, hd, Nq, Nk, dt;
     float c; /* scale log2 e */
-    int wm, tiles, splits, heads_first;
+    int few, wm, tiles, splits, heads_first;
     long items;
     float *part; /* [split][unit][grp Nq] rows of hd sums, then (m, sum) */
     long part_ml;
