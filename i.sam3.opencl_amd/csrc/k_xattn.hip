@@ -28,19 +28,20 @@
 #include "k_xattn.h"
 
 /* DP: head width padded to 32, 64, 128 or 256. WM waves share the rows of a
- * workgroup, 4 / WM the keys of a tile. TK: keys of a tile. ST: tiles in LDS,
- * ST - 1 of them ahead. VEC: the rows of all operands are whole 16-byte
- * pieces. */
+ * workgroup, the rest of its four the keys of a tile; WM = 8 is eight waves, each
+ * with rows of its own. TK: keys of a tile. ST: tiles in LDS, ST - 1 of them
+ * ahead. VEC: the rows of all operands are whole 16-byte pieces. */
 template <int DT, int DP, int WM, int TK, int ST, int OCC, bool VEC>
-__global__ __launch_bounds__(256, OCC) void k_xattn(const struct xattn_desc a)
+__global__ __launch_bounds__(WM == 8 ? 512 : 256, OCC) void k_xattn(const struct xattn_desc a)
 {
     constexpr int S = xt<DT>::size;
-    constexpr int WK = 4 / WM;
+    constexpr int NW = WM == 8 ? 8 : 4;
+    constexpr int WK = NW / WM;
     constexpr int KW = TK / WK;          /* keys of a tile that a wave takes */
     constexpr int NB = KW / 32;          /* 32-key blocks of them */
     constexpr int RB = DP * S;           /* bytes of a row */
     constexpr int CH = RB / 16;          /* 16-byte chunks of a row */
-    constexpr int NI = TK * RB / 4096;   /* copies of a wave for K or V: 1 KiB each */
+    constexpr int NI = TK * RB / (1024 * NW); /* copies of a wave for K or V: 1 KiB each */
     constexpr int MERGE = WK > 1 ? 4 * 32 * (DP + 4) * 4 + 4 * 32 * 8 : 0;
     typedef row_k<RB> rk;
     typedef row_v<RB, DT> rv;
@@ -729,8 +730,8 @@ static int padded(int hd)
  *   12 heads of 64, 447 rows, 1500 keys: batch 64 207 / 217 / 367, batch 4 22.8 /
  *   21.3 / 23.3, batch 1 - / 16.0 / 11.7 (15.0 with two splits of wm 1);
  *   8 heads of 64, 1000 x 1000: 16.5 / 12.4 / 9.7 (best split 14.5);
- *   one head of 256, 5184 x 20751, bf16: 144 with 12 splits, 192 with 16 (a
- *   workgroup too many per compute unit), 175 with 8, wm 2 236.
+ *   one head of 256, 5184 x 20751, bf16: 138 with 12 splits, 192 with 16 (a
+ *   workgroup too many per compute unit), 175 with 8, wm 2 236, wm 8 130.
  * So: as many rows as still give two workgroups per compute unit, or one and a
  * quarter with wm 2; splits only where even the least rows leave half of the
  * compute units idle, and then two workgroups for each.
@@ -764,7 +765,32 @@ static void plan(struct xattn_desc *d)
     }
     if (!d->vec)
         wm = rb >= 1024 ? 4 : 2;
-    else if (d->Nk > 256) {
+    else if (d->dt != DT_F32 && rb >= 256 && rows >= (rb == 256 ? 1024 : 256) && d->Nk > 256) {
+        /* The copies into LDS are what such heads wait for (6 to 8 TB/s): 256 rows
+         * share them, one workgroup of eight waves per compute unit and as many
+         * splits as make one for each, unless they get short. us, against the
+         * rules below: 5184 x 5184 with 8, 4, 2 heads of 128 127 / 71 / 45 and
+         * 154 / 85 / 60; 5184 x 20751, one head of 256 130 and 138; 447 x 1500,
+         * 64 heads of 256 83 and 97. But with heads of 128 2048 x 2048, 8 heads
+         * in splits of 512 keys 37 and 31, 512 x 2048, 64 heads 56 and 48. */
+        const long tiles = (rows + 255) / 256, wg = d->units * tiles;
+        long want = cu / wg, rounds;
+
+        if (want > d->Nk / (rb == 256 ? 768 : 384))
+            want = d->Nk / (rb == 256 ? 768 : 384);
+        if (want < 1)
+            want = 1;
+        rounds = (wg * want + cu - 1) / cu;
+        /* Where more than four in ten compute units would be idle: below. */
+        if (10 * wg * want >= 6 * cu * rounds) {
+            d->wm = 8;
+            d->tiles = (int)tiles;
+            d->splits = (int)want;
+            d->heads_first = 0;
+            return;
+        }
+    }
+    if (d->vec && d->Nk > 256) {
         const int most_rows = wm;
         long want = 2 * cu;
 
@@ -772,7 +798,7 @@ static void plan(struct xattn_desc *d)
             wm = 2;
         if (wm == 2 && least == 1 && WG(2) < cu + cu / 4)
             wm = 1;
-        if (rows <= 64 ? WG(wm) < 2 * cu : WG(wm) <= cu / 2) {
+        if (rows <= 64 ? WG(wm) < 2 * cu : WG(wm) < cu / 2) {
             wm = most_rows;
             if (rows <= 64)
                 want = 4 * cu;
@@ -809,7 +835,8 @@ static int run(const struct xattn_desc *d, hipStream_t s)
     const unsigned grid = d->heads_first ? item_grid(d->tiles, d->units)
                                          : item_grid(d->units * d->splits, d->tiles);
 
-    hipLaunchKernelGGL((k_xattn<DT, DP, WM, TK, ST, OCC, VEC>), dim3(grid), dim3(256), 0, s, *d);
+    hipLaunchKernelGGL((k_xattn<DT, DP, WM, TK, ST, OCC, VEC>), dim3(grid),
+                       dim3(WM == 8 ? 512 : 256), 0, s, *d);
     return hipGetLastError();
 }
 
@@ -833,6 +860,11 @@ template <int DT, int DP> static int run_wm(const struct xattn_desc *d, hipStrea
             return run<DT, DP, 4, 32, 2, 1, false>(d, s);
         else
             return run<DT, DP, 2, 64, 2, 1, false>(d, s);
+    }
+    if (d->wm == 8) {
+        if constexpr (DT != DT_F32 && RB >= 256)
+            return run<DT, DP, 8, RB == 256 ? 64 : 32, 3, 2>(d, s);
+        return hipErrorInvalidValue;
     }
     /* LDS of a tile of 64 keys: 8, 16, 32 KiB for rows of 64, 128, 256 bytes. */
     if (d->wm == 4) {

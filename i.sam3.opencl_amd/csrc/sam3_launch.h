@@ -358,7 +358,7 @@ struct xattn_desc {
     const unsigned char *kmask;
     int units, kvh, grp, hd, Nq, Nk, dt;
     float c; /* scale log2 e */
-    int few, wide, wm, tiles, splits, heads_first;
+    int few, wm, tiles, splits, heads_first;
     float *part; /* [split][unit][grp Nq] rows of hd sums, then (m, sum) */
     long part_ml;
 };
@@ -367,8 +367,6 @@ struct xattn_desc {
  * want to); with less, or NULL, one workgroup walks all keys of its rows. */
 size_t xattn_ws(struct xattn_desc *d);
 int launch_xattn(struct xattn_desc *d, void *ws, size_t ws_bytes, void *stream);
-/* 256 rows per workgroup, heads of 128 to 256 halves or bf16 (d->wide). */
-int launch_xattn_wide(const struct xattn_desc *d, void *stream);
 
 /* ------------------------------------------------ rotary positions */
 

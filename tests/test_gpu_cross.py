@@ -218,3 +218,19 @@ def test_far_offsets(hip, env):
     assert (np.abs(got - o) <= sc.cross_bound(o, av, top, prod, D, nk, sc.F16, vv)).all()
     for x in (big, Q, O):
         be.release(x)
+
+
+@pytest.mark.parametrize("t", ["f16", "bf16"])
+@pytest.mark.parametrize("D,H,KV,nq,nk", [
+    (128, 2, 1, 600, 1100), (128, 2, 2, 10000, 2000), (128, 4, 2, 5050, 2000), (72, 40, 40, 1100, 300),
+    (256, 1, 1, 1030, 1537), (256, 80, 80, 257, 261), (256, 16, 8, 550, 2400), (200, 4, 4, 1291, 1090)])
+def test_many_rows_wide_heads(hip, env, t, D, H, KV, nq, nk):
+    """256 rows per workgroup: with and without splits, shared heads, masks,
+    lengths that end inside a tile or before it."""
+    g = np.random.default_rng(D)
+    nb = 8 if D == 200 else 1
+    check(hip, env, D, sc.TYPES[t], nb, H, KV, D, nq, nk)
+    mask = (g.random((nb, nk)) < 0.5).astype(np.uint8)
+    check(hip, env, D + 1, sc.TYPES[t], nb, H, KV, D, nq, nk, kmask=mask, klen=[nk - 33] * nb,
+          qlen=[nq - 300] * nb)
+    check(hip, env, D + 2, sc.TYPES[t], nb, H, KV, D, nq, nk, klen=[65] * nb)
