@@ -62,8 +62,8 @@ template <int N> __global__ __launch_bounds__(256) void k_rope_table(const struc
 #pragma unroll
     for (int e = 0; e < N; e++)
         f[e] = d.turns[u * N + e];
-    for (int p = blockIdx.y * per + t / min(units, 256); p < d.npos; p += gridDim.y * per) {
-        const int pos = d.pos ? d.pos[p] : p;
+    for (long p = blockIdx.y * per + t / min(units, 256); p < d.npos; p += gridDim.y * per) {
+        const int pos = d.pos ? d.pos[p] : (int)p;
         float v[2 * N];
 
 #pragma unroll
@@ -74,7 +74,7 @@ template <int N> __global__ __launch_bounds__(256) void k_rope_table(const struc
             v[2 * e] = cs.x * d.mul;
             v[2 * e + 1] = cs.y * d.mul;
         }
-        float *const o = d.table + 2 * ((long)p * d.pairs + u * N);
+        float *const o = d.table + 2 * (p * d.pairs + u * N);
 
         if constexpr (N == 2)
             STORE((f32x4 *)o, (f32x4{v[0], v[1], v[2], v[3]}));

@@ -168,6 +168,14 @@ template <int RB, int DT> struct row_v {
     }
 };
 
+/* Lanes read what others of their wave have written to LDS: served in order,
+ * which the compiler has to keep. */
+__device__ __forceinline__ void wave_lds_order()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 /* The same copy as g2lds16 from an address of each lane's own. */
 __device__ __forceinline__ void g2lds16_at(const void *src, unsigned lds)
 {

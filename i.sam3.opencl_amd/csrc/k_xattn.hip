@@ -212,6 +212,7 @@ __global__ __launch_bounds__(WM == 8 ? 512 : 256, OCC) void k_xattn(const struct
             for (int c = l; c < KW * CH; c += 64)
                 if (!(keep >> (c / CH) & 1))
                     *(u32x4 *)(ldv + rv::at(c / CH) + 16 * (c % CH)) = u32x4{0, 0, 0, 0};
+            wave_lds_order();
         }
         float mx = s[0][0];
 
@@ -544,6 +545,7 @@ __global__ __launch_bounds__(256, 2) void k_xattn_few(const struct xattn_desc a)
 #pragma unroll
         for (int i = 0; i < CH / 2; i++)
             *(u32x4 *)(own + (i * (64 / CH) + l / CH) * QP + 16 * (l % CH)) = q[i];
+        wave_lds_order();
         load_q(blk + step);
 #pragma unroll
         for (int n = 0; n < NB; n++)
@@ -621,6 +623,7 @@ __global__ __launch_bounds__(256, 2) void k_xattn_few(const struct xattn_desc a)
 #pragma unroll
         for (int d = 0; d < DP / 32; d++)
             put_block<DT, true>(own + lr * QP, 32 * d, DP, h, o[d], inv);
+        wave_lds_order();
 #pragma unroll
         for (int i = 0; i < CH / 2; i++) {
             const int r = i * (64 / CH) + l / CH;
@@ -630,6 +633,7 @@ __global__ __launch_bounds__(256, 2) void k_xattn_few(const struct xattn_desc a)
                 __builtin_nontemporal_store(
                     v, (u32x4 *)((char *)a.O + row_at(blk, i, a.oo, a.os0, a.os1, a.old)));
         }
+        wave_lds_order();
     }
 }
 

@@ -1602,13 +1602,61 @@ static void opnd_span(struct opnd o, int nb, int heads, long rows, long cols, lo
     *last = o.off + (nb - 1) * o.s0 + (heads - 1) * o.s1 + (rows - 1) * (long)o.ld + cols - 1;
 }
 
-/* Do two operands (spans as above) share memory? */
-static int spans_meet(struct opnd a, const long *sa, struct opnd b, const long *sb)
+/* Columns that the operand's elements take modulo ld, from its first one on,
+ * or 0 where they are not an interval: batches and heads lie whole rows apart,
+ * or side by side in a row. */
+static long opnd_columns(struct opnd o, int nb, int heads, long cols)
 {
-    const long za = elem_size(a.buf->dtype), zb = elem_size(b.buf->dtype);
-    const char *pa = a.buf->ptr, *pb = b.buf->ptr;
+    if (o.ld <= 0)
+        return 0;
+    if (nb > 1 && o.s0 % o.ld)
+        cols += (nb - 1) * o.s0;
+    if (heads > 1 && o.s1 % o.ld)
+        cols += (heads - 1) * o.s1;
+    return cols <= o.ld ? cols : 0;
+}
 
-    return pa + sa[0] * za < pb + (sb[1] + 1) * zb && pb + sb[0] * zb < pa + (sa[1] + 1) * za;
+/* Do two operands of one element type (nb batches x heads of rows x cols each)
+ * share memory? No where their spans are apart, or their rows' columns are, as
+ * those of two slices of a wider matrix. */
+static int opnds_meet(struct opnd a, int ha, long ra, struct opnd b, int hb, long rb, int nb,
+                      long cols)
+{
+    const long z = elem_size(a.buf->dtype), ld = a.ld * z;
+    const char *pa = a.buf->ptr, *pb = b.buf->ptr;
+    long sa[2], sb[2], wa, wb, at;
+
+    opnd_span(a, nb, ha, ra, cols, &sa[0], &sa[1]);
+    opnd_span(b, nb, hb, rb, cols, &sb[0], &sb[1]);
+    if (pa + sa[0] * z >= pb + (sb[1] + 1) * z || pb + sb[0] * z >= pa + (sa[1] + 1) * z)
+        return 0;
+    wa = opnd_columns(a, nb, ha, cols) * z;
+    wb = opnd_columns(b, nb, hb, cols) * z;
+    if (a.ld != b.ld || !wa || !wb)
+        return 1;
+    /* b's first column, from a's on. */
+    at = ((pb + sb[0] * z) - (pa + sa[0] * z)) % ld;
+    if (at < 0)
+        at += ld;
+    return at < wa || at + wb > ld;
+}
+
+/* True if n bytes of m (none if NULL) lie apart from operand o; fatal
+ * otherwise. */
+static int opnd_apart(const char *op, const char *name, struct opnd o, int nb, int heads, long rows,
+                      long cols, const char *mname, hipb_mem m, size_t n)
+{
+    const char *p = o.buf->ptr, *q = m ? m->ptr : NULL;
+    long so[2];
+
+    if (!m || !n)
+        return 1;
+    opnd_span(o, nb, heads, rows, cols, &so[0], &so[1]);
+    if (p + so[0] * elem_size(o.buf->dtype) >= q + n ||
+        q >= p + (so[1] + 1) * elem_size(o.buf->dtype))
+        return 1;
+    hipb_fatal("%s: %s overlaps %s", op, name, mname);
+    return 0;
 }
 
 /* True if no two elements of an output operand (nb x heads x rows x cols) are
@@ -1718,10 +1766,11 @@ static int xattn_shape(struct xattn_desc *d, const char *op, int nb, int heads, 
         hipb_fatal("%s: unknown element type %d", op, dtype);
         return 0;
     }
-    /* Rows and work items are counted in 32 bits. */
-    if ((long)nb * heads > 1L << 22 || (long)heads / kv_heads * Nq > 0x7fffffffL - 128 ||
+    /* Rows, keys and work items are counted in 32 bits. */
+    if ((long)nb * heads > 1L << 22 || Nk > 1 << 30 || (long)heads / kv_heads * Nq > 0x7fffffffL - 128 ||
         (double)nb * heads * Nq > 6.4e7) {
-        hipb_fatal("%s: too many rows (nb=%d heads=%d Nq=%d)", op, nb, heads, Nq);
+        hipb_fatal("%s: too many rows or keys (nb=%d heads=%d Nq=%d Nk=%d)", op, nb, heads, Nq,
+                   Nk);
         return 0;
     }
     memset(d, 0, sizeof(*d));
@@ -1758,7 +1807,6 @@ void cross_attend(struct sam_model *m, int nb, int heads, int kv_heads, int hd, 
     static const char op[] = "cross_attend";
     struct hipb_backend *be = m->hip;
     struct xattn_desc d;
-    long so[2], si[2];
     const struct opnd *in[3] = {&Q, &K, &V};
     size_t ws_bytes, need;
     void *wp;
@@ -1775,7 +1823,7 @@ void cross_attend(struct sam_model *m, int nb, int heads, int kv_heads, int hd, 
                    K.buf->dtype, V.buf->dtype, O.buf->dtype);
         return;
     }
-    if (!(scale > 0.0f) || isinf(scale)) {
+    if (!(scale > 0.0f) || isinf(scale * LOG2E_HOST)) {
         hipb_fatal("%s: scale %g is not positive and finite", op, (double)scale);
         return;
     }
@@ -1791,26 +1839,32 @@ void cross_attend(struct sam_model *m, int nb, int heads, int kv_heads, int hd, 
         hipb_fatal("%s: rows of K or V are more than 16 MiB apart", op);
         return;
     }
-    opnd_span(O, nb, heads, Nq, hd, &so[0], &so[1]);
-    for (i = 0; i < 3; i++) {
-        if (i && Nk == 0)
-            break;
-        opnd_span(*in[i], nb, i ? kv_heads : heads, i ? Nk : Nq, hd, &si[0], &si[1]);
-        if (spans_meet(O, so, *in[i], si)) {
+    for (i = 0; i < (Nk ? 3 : 1); i++)
+        if (opnds_meet(O, heads, Nq, *in[i], i ? kv_heads : heads, i ? Nk : Nq, nb, hd)) {
             hipb_fatal("%s: O overlaps %c", op, "QKV"[i]);
             return;
         }
-    }
     if ((qlen && !bytes_ok(op, "qlen", qlen, 4 * (size_t)nb)) ||
         (klen && !bytes_ok(op, "klen", klen, 4 * (size_t)nb)) ||
-        (kmask && !bytes_ok(op, "kmask", kmask, (size_t)nb * Nk)))
+        (kmask && !bytes_ok(op, "kmask", kmask, (size_t)nb * Nk)) ||
+        !opnd_apart(op, "O", O, nb, heads, Nq, hd, "qlen", qlen, 4 * (size_t)nb) ||
+        !opnd_apart(op, "O", O, nb, heads, Nq, hd, "klen", klen, 4 * (size_t)nb) ||
+        !opnd_apart(op, "O", O, nb, heads, Nq, hd, "kmask", kmask, (size_t)nb * Nk))
         return;
     d.vec = hd * elem_size(d.dt) % 16 == 0 && opnd_vec(Q, nb, heads, Nq) &&
             opnd_vec(K, nb, kv_heads, Nk) && opnd_vec(V, nb, kv_heads, Nk) &&
             opnd_vec(O, nb, heads, Nq);
     need = xattn_ws(&d);
-    if (!workspace(be, op, ws, need, &wp, &ws_bytes))
+    if (ws && (!opnd_apart(op, "Q", Q, nb, heads, Nq, hd, "ws", ws, need) ||
+               (Nk && !opnd_apart(op, "K", K, nb, kv_heads, Nk, hd, "ws", ws, need)) ||
+               (Nk && !opnd_apart(op, "V", V, nb, kv_heads, Nk, hd, "ws", ws, need)) ||
+               !opnd_apart(op, "O", O, nb, heads, Nq, hd, "ws", ws, need)))
         return;
+    old = device_enter(be);
+    if (!workspace(be, op, ws, need, &wp, &ws_bytes)) {
+        device_leave(be, old);
+        return;
+    }
     d.Q = Q.buf->ptr;
     d.qo = Q.off;
     d.qs0 = Q.s0;
@@ -1835,7 +1889,6 @@ void cross_attend(struct sam_model *m, int nb, int heads, int kv_heads, int hd, 
     d.klen = klen ? klen->ptr : NULL;
     d.kmask = kmask ? kmask->ptr : NULL;
     d.c = scale * LOG2E_HOST;
-    old = device_enter(be);
     hipb_run_begin(be);
     err = launch_xattn(&d, wp, ws_bytes, be->stream);
     hipb_run_end(be, err, op, 4.0 * nb * heads * (double)Nq * Nk * hd);
@@ -1872,6 +1925,11 @@ void rope_table(struct sam_model *m, hipb_mem table, int npos, hipb_mem pos, int
         return;
     if ((uintptr_t)table->ptr % 8) {
         hipb_fatal("%s: table is not 8-byte aligned", op);
+        return;
+    }
+    if (pos && (char *)pos->ptr < (char *)table->ptr + 4 * (size_t)npos * rot &&
+        (char *)table->ptr < (char *)pos->ptr + 4 * (size_t)npos) {
+        hipb_fatal("%s: table overlaps pos", op);
         return;
     }
     if ((long)npos * (rot / 2) > GRID_MAX - 256) {
@@ -1916,7 +1974,6 @@ void rope_rows(struct sam_model *m, int nb, int heads, int rows, int hd, int rot
     static const char op[] = "rope_rows";
     struct hipb_backend *be = m->hip;
     struct rope_rows_desc d;
-    long sx[2], sy[2];
     int err, old, v, same;
 
     if (nb < 0 || heads < 1 || rows < 0 || hd < 2 || rot < 2 || rot % 2 || rot > hd || npos < 1 ||
@@ -1928,7 +1985,7 @@ void rope_rows(struct sam_model *m, int nb, int heads, int rows, int hd, int rot
     }
     if (nb == 0 || rows == 0)
         return;
-    if ((long)nb * heads > 0x7fffffffL) {
+    if ((long)nb * heads > 1L << 30) {
         hipb_fatal("%s: too many heads (nb=%d heads=%d)", op, nb, heads);
         return;
     }
@@ -1947,12 +2004,13 @@ void rope_rows(struct sam_model *m, int nb, int heads, int rows, int hd, int rot
                (char *)Y.buf->ptr + Y.off * elem_size(Y.buf->dtype) &&
            (rows == 1 || X.ld == Y.ld) && (nb == 1 || X.s0 == Y.s0) &&
            (heads == 1 || X.s1 == Y.s1);
-    opnd_span(X, nb, heads, rows, hd, &sx[0], &sx[1]);
-    opnd_span(Y, nb, heads, rows, hd, &sy[0], &sy[1]);
-    if (!same && spans_meet(X, sx, Y, sy)) {
+    if (!same && opnds_meet(X, heads, rows, Y, heads, rows, nb, hd)) {
         hipb_fatal("%s: Y overlaps X and is not X", op);
         return;
     }
+    if (!opnd_apart(op, "Y", Y, nb, heads, rows, hd, "table", table, 4 * (size_t)npos * rot) ||
+        !opnd_apart(op, "Y", Y, nb, heads, rows, hd, "pos", pos, 4 * (size_t)nb * rows))
+        return;
     if ((double)nb * rows * hd > 4e9) {
         hipb_fatal("%s: too many rows (nb=%d rows=%d)", op, nb, rows);
         return;
@@ -2028,7 +2086,7 @@ void groupnorm(struct sam_model *m, int nb, long rows, int C, int groups, struct
     static const char op[] = "groupnorm";
     struct hipb_backend *be = m->hip;
     struct groupnorm_desc d;
-    long sx[2], sy[2], v;
+    long v;
     size_t ws_bytes, need;
     void *wp;
     int err, old, same;
@@ -2058,15 +2116,21 @@ void groupnorm(struct sam_model *m, int nb, long rows, int C, int groups, struct
     same = (char *)X.buf->ptr + X.off * elem_size(d.dt) ==
                (char *)Y.buf->ptr + Y.off * elem_size(d.dt) &&
            (rows == 1 || X.ld == Y.ld) && (nb == 1 || X.s0 == Y.s0);
-    opnd_span(X, nb, 1, rows, C, &sx[0], &sx[1]);
-    opnd_span(Y, nb, 1, rows, C, &sy[0], &sy[1]);
-    if (!same && spans_meet(X, sx, Y, sy)) {
+    if (!same && opnds_meet(X, 1, rows, Y, 1, rows, nb, C)) {
         hipb_fatal("%s: Y overlaps X and is not X", op);
         return;
     }
     need = groupnorm_ws_bytes(&d);
-    if (!workspace(be, op, ws, need, &wp, &ws_bytes))
+    if (!opnd_apart(op, "Y", Y, nb, 1, rows, C, "g", g, 4 * (size_t)C) ||
+        !opnd_apart(op, "Y", Y, nb, 1, rows, C, "b", b, 4 * (size_t)C) ||
+        (ws && (!opnd_apart(op, "X", X, nb, 1, rows, C, "ws", ws, need) ||
+                !opnd_apart(op, "Y", Y, nb, 1, rows, C, "ws", ws, need))))
         return;
+    old = device_enter(be);
+    if (!workspace(be, op, ws, need, &wp, &ws_bytes)) {
+        device_leave(be, old);
+        return;
+    }
     d.X = X.buf->ptr;
     d.xo = X.off;
     d.xs0 = X.s0;
@@ -2087,7 +2151,6 @@ void groupnorm(struct sam_model *m, int nb, long rows, int C, int groups, struct
             ((uintptr_t)X.buf->ptr | (uintptr_t)Y.buf->ptr) % (v * elem_size(d.dt)) == 0)
             break;
     d.vec = (int)v;
-    old = device_enter(be);
     hipb_run_begin(be);
     err = launch_groupnorm(&d, wp, ws_bytes, be->stream);
     hipb_run_end(be, err, op, 0.0);

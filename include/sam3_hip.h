@@ -409,7 +409,10 @@ void sam_trunk_graph(struct sam_model *m, int enable);
  * or wider, results are rounded once. (P of half and bf16 attention is rounded
  * to the operands' type, as the product with V takes it.) Integers, positions
  * and masks lie in plain buffers (hipb_alloc). The operators queue kernels
- * only and may be captured; see `ws` for their workspace. */
+ * only and may be captured; see `ws` for their workspace. What they write lies
+ * apart from all that they read (rows of a matrix may have columns of both),
+ * unless in place is said; calls that break this, reach past a buffer, write
+ * an element twice or exceed a size below are errors, and queue nothing. */
 
 /* Cross attention: for batch b < nb, head h < heads and query i < qlen[b]
  * (Nq where qlen is NULL),
@@ -422,7 +425,8 @@ void sam_trunk_graph(struct sam_model *m, int enable);
  * bytes. What stands in masked keys and values, or behind the lengths, is
  * not used, NaN or infinity neither; a query without a key, or whose scores
  * are all minus infinity, gives zeros; rows of O behind qlen are left as they
- * are. scale is positive.
+ * are. scale is positive. At most 2^22 heads in all batches, 6.4e7 of their
+ * rows, 2^30 keys, and 16 MiB from one row of K or V to the next.
  * Few rows over many keys are split over workgroups, whose partial sums go to
  * ws: at least cross_attend_ws bytes of the caller's, which calls that may
  * overlap (other streams, graphs) must not share; or NULL for the backend's
@@ -473,8 +477,9 @@ void rope_table(struct sam_model *m, hipb_mem table, int npos, hipb_mem pos,
  * s0 + h s1 + r ld. Row r of batch b has position pos[b][r] (int32 [nb][rows]),
  * or (pos0 + r) % npos where pos is NULL; a row whose position is outside 0 ..
  * npos - 1 (-1, say) is not rotated. Y is X (in place) or does not overlap
- * it; both have one element type. The inverse rotation (the gradient) is
- * that of a table with the sines negated. */
+ * it; both have one element type. At most 2^30 heads in all batches and 4e9
+ * columns of a head over all rows. The inverse rotation (the gradient) is that
+ * of a table with the sines negated. */
 void rope_rows(struct sam_model *m, int nb, int heads, int rows, int hd,
                int rot, int layout, struct opnd X, struct opnd Y,
                hipb_mem table, int npos, hipb_mem pos, long pos0);
@@ -484,8 +489,8 @@ void rope_rows(struct sam_model *m, int nb, int heads, int rows, int hd,
 /* Group norm of channels-last rows: nb batches (s0 apart; s1 is not used) of
  * rows of C channels, mean and biased variance per batch and group of C /
  * groups channels over all rows, y = act((x - mean) / sqrt(var + eps) g + b);
- * g and b hold C floats (NULL: ones, zeros). Y may be X, or does not overlap
- * it; both have one element type. ws as in cross_attend, groupnorm_ws bytes. */
+ * g and b hold C floats (NULL: ones, zeros). At most 65535 batches and 4096
+ * groups. Y may be X, or does not overlap it; both have one element type. ws as in cross_attend, groupnorm_ws bytes. */
 void groupnorm(struct sam_model *m, int nb, long rows, int C, int groups,
                struct opnd X, struct opnd Y, hipb_mem g, hipb_mem b, float eps,
                int act, hipb_mem ws);

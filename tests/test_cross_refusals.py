@@ -103,6 +103,57 @@ def test_cross_too_many_rows(hip):
         cross(hip, nb=1 << 20, heads=8, kv_heads=8)
     with pytest.raises(hip.Sam3HipError, match="too many rows"):
         cross(hip, nb=64, heads=64, kv_heads=64, Nq=1 << 20)
+    with pytest.raises(hip.Sam3HipError, match="too many rows or keys"):
+        cross(hip, Nk=(1 << 30) + 1)
+
+
+def test_cross_overlaps(hip):
+    """Whatever the call writes lies apart from whatever it reads."""
+    o = hip.bmat(mem(hip, 100000, 0, 3 << 20), 0, 128, 1024, 32)
+    for n, k in (("qlen", 8), ("klen", 8), ("kmask", 14)):
+        with pytest.raises(hip.Sam3HipError, match="cross_attend: O overlaps " + n):
+            cross(hip, O=o, **{n: mem(hip, k, 0, (3 << 20) + 4096)})
+    # Few rows over many keys: split, with sums in ws.
+    q = hip.bmat(mem(hip, 100000), 0, 128, 0, 0)
+    k = hip.bmat(mem(hip, 4000 * 128, 0, 1 << 24), 0, 128, 0, 0)
+    v = hip.bmat(mem(hip, 4000 * 128, 0, 1 << 26), 0, 128, 0, 0)
+    o = hip.bmat(mem(hip, 100000, 0, 1 << 28), 0, 128, 0, 0)
+    for n, at in (("Q", 0), ("K", 1 << 24), ("V", 1 << 26), ("O", 1 << 28)):
+        with pytest.raises(hip.Sam3HipError, match=f"cross_attend: {n} overlaps ws"):
+            cross(hip, nb=1, heads=1, kv_heads=1, Nq=1, Nk=4000, Q=q, K=k, V=v, O=o,
+                  ws=mem(hip, 1 << 20, 0, at))
+    # Columns of one matrix that meet (8 of them), on either side and around its end.
+    for at, other in ((0, 24), (24, 0), (104, 0)):
+        buf = mem(hip, 100000, 0, 8 << 20)
+        with pytest.raises(hip.Sam3HipError, match="O overlaps Q"):
+            cross(hip, heads=1, kv_heads=1, Q=hip.bmat(buf, at, 128, 1024, 0),
+                  O=hip.bmat(buf, other if at != 104 else 128 * 8, 128, 1024, 0))
+
+
+def test_other_overlaps(hip):
+    x = hip.bmat(mem(hip, 10000), 0, 64, 640, 0)
+    y = hip.bmat(mem(hip, 10000, 0, 1 << 20), 0, 64, 640, 0)
+    far = mem(hip, 10000, 0, 1 << 24)
+    inside = mem(hip, 10000, 0, (1 << 20) + 1024)
+
+    def bad(msg, f, *a, **kw):
+        with pytest.raises(hip.Sam3HipError, match=msg):
+            f(Model(hip), *a, **kw)
+
+    bad("rope_rows: Y overlaps table", hip.rope_rows, 2, 1, 9, 64, 64, 0, x, y, inside, 9)
+    bad("rope_rows: Y overlaps pos", hip.rope_rows, 2, 1, 9, 64, 64, 0, x, y, far, 9, pos=inside)
+    bad("rope_rows: too many heads", hip.rope_rows, 2, 1 << 30, 9, 64, 64, 0, x, y, far, 9)
+    bad("rope_table: table overlaps pos", hip.rope_table, far, 9,
+        mem(hip, 100, 0, (1 << 24) + 64), 64)
+    bad("groupnorm: Y overlaps g", hip.groupnorm, 2, 9, 64, 8, x, y, g=inside, b=far)
+    bad("groupnorm: Y overlaps b", hip.groupnorm, 2, 9, 64, 8, x, y, g=far, b=inside)
+    big = hip.bmat(mem(hip, 1 << 20), 0, 64, 0, 0)
+    out = hip.bmat(mem(hip, 1 << 20, 0, 1 << 26), 0, 64, 0, 0)
+    for n, at in (("X", 0), ("Y", 1 << 26)):
+        bad(f"groupnorm: {n} overlaps ws", hip.groupnorm, 1, 1 << 14, 64, 8, big, out,
+            ws=mem(hip, 1 << 20, 0, at))
+    bad("rope_rows: Y overlaps X", hip.rope_rows, 2, 1, 9, 64, 32, 0, hip.bmat(far, 0, 128, 1280, 0),
+        hip.bmat(far, 32, 128, 1280, 0), mem(hip, 1000), 9)
 
 
 def test_empty_calls_queue_nothing(hip):

@@ -462,3 +462,37 @@ def test_two_backends(hip, env):
     lim = sc.cross_bound(want, av, top, prod, 64, 5000, sc.F16, ops[0][2].values)
     assert (np.abs(a - want) <= lim).all() and np.array_equal(a, b)
     be2.free()
+
+
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("D", [32, 20])
+def test_slices_of_one_matrix(hip, env, t, D):
+    """What is written may be columns of the matrix that is read: the results
+    are those of a buffer apart, the other columns stay."""
+    be, m = env
+    dt, nb, H, n = sc.TYPES[t], 2, 2, 77
+    g = np.random.default_rng(D)
+    W = H * D
+    x, _ = sc.store(g.standard_normal((nb, n, 4 * W), np.float32), dt)
+    tab = be.alloc(4 * n * D)
+    hip.rope_table(m, tab, n, None, D)
+
+    def calls(run):
+        src, out = be.upload_typed(x, dt), be.alloc_typed(x.size, dt)
+        one = be.upload_typed(x, dt)
+        rows = [hip.bmat(b, c * W, 4 * W, n * 4 * W, D)
+                for b, c in ((src, 0), (src, 1), (src, 2), (out, 3), (one, 0), (one, 1), (one, 2),
+                             (one, 3))]
+        run(*rows[:4])
+        run(*rows[4:])
+        a, b = (np.frombuffer(be.read(z).tobytes(), x.dtype).reshape(x.shape) for z in (out, one))
+        for z in (src, out, one):
+            be.release(z)
+        assert (a[..., 3 * W:] == b[..., 3 * W:]).all()
+        assert (b[..., :3 * W] == x[..., :3 * W]).all() and not (b == x).all()
+
+    calls(lambda q, k, v, o: hip.cross_attend(m, nb, H, H, D, n, n, q, k, v, o))
+    for layout in (hip.ROPE_PAIRS, hip.ROPE_HALVES):
+        calls(lambda q, k, v, o: hip.rope_rows(m, nb, H, n, D, D, layout, q, o, tab, n))
+    calls(lambda q, k, v, o: hip.groupnorm(m, nb, n, W, 4, q, o))
+    be.release(tab)
