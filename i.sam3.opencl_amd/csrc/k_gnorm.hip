@@ -14,10 +14,11 @@
 
 #define ACT_SILU_K 3
 /* Threads of the kernels that share a batch entry's rows, and vectors that each
- * has under way. us of both kernels at 82944 rows of 256 floats: 512 threads,
- * two workgroups per compute unit for the sums, one for the rest 17.4 + 28.3;
- * 256 threads and four 15.8 + 37; 1024 and one 20.0 + 28.5 (every workgroup of
- * the second kernel adds up all sums of its batch entry). */
+ * has under way. us of both kernels at 82944 rows of 256 floats, the second
+ * from the first rows on: 512 threads, two workgroups per compute unit for the
+ * sums, one for the rest 17.4 + 28.3; 256 threads and four 15.8 + 37; 1024 and
+ * one 20.0 + 28.5 (every workgroup of the second kernel adds up all sums of
+ * its batch entry). */
 #define TH 512
 #define AHEAD_SUMS 4
 #define AHEAD_APPLY 8
@@ -254,12 +255,13 @@ __global__ __launch_bounds__(T) void k_gn_group(const struct groupnorm_desc d)
     });
 }
 
-/* This workgroup's rows of batch entry blockIdx.y. */
-__device__ __forceinline__ void chunk_rows(const struct groupnorm_desc &d, long *r0, long *r1)
+/* Chunk i of n of a batch entry's rows. */
+__device__ __forceinline__ void chunk_rows(const struct groupnorm_desc &d, int n, int i, long *r0,
+                                           long *r1)
 {
-    const long per = (d.rows + gridDim.x - 1) / gridDim.x;
+    const long per = (d.rows + n - 1) / n;
 
-    *r0 = min(d.rows, blockIdx.x * per);
+    *r0 = min(d.rows, i * per);
     *r1 = min(d.rows, *r0 + per);
 }
 
@@ -305,17 +307,21 @@ template <int DT, int V, int AHEAD> struct stream {
 /* Sums of a chunk of rows, per group. A thread keeps one column of V channels
  * (or, where a row has more than TH of them, one of each block of TH) and
  * walks every (TH / columns)-th row; a group's threads are then added in
- * order. */
+ * order. Where the number of chunks is a multiple of 16, chunks 2 i and 2 i + 1
+ * are summed on the XCD (workgroup index mod 8) whose workgroup i of k_gn_apply
+ * takes both. */
 template <int DT, int V>
 __global__ __launch_bounds__(TH) void k_gn_stats(const struct groupnorm_desc d)
 {
     __shared__ double2 red[TH];
     const int t = threadIdx.x, b = blockIdx.y;
     const int cv = d.C / V, gv = d.C / d.groups / V;
-    double2 *const part = (double2 *)d.part + (long)b * d.groups * d.chunks + blockIdx.x;
+    const int i = blockIdx.x;
+    const int chunk = d.chunks % 16 ? i : (i & ~15) + 2 * (i & 7) + (i >> 3 & 1);
+    double2 *const part = (double2 *)d.part + (long)b * d.groups * d.chunks + chunk;
     long r0, r1;
 
-    chunk_rows(d, &r0, &r1);
+    chunk_rows(d, d.chunks, chunk, &r0, &r1);
     const int w = min(cv, TH), lanes = TH / w;
     const int col = t % w, row = t / w;
 
@@ -406,7 +412,11 @@ __global__ __launch_bounds__(256) void k_gn_sums(const struct groupnorm_desc d)
         ((struct stat *)d.stats)[b * d.groups + g] = s;
 }
 
-/* The chunk's rows normalised by mean and deviation of each group. */
+/* The rows of two chunks normalised by mean and deviation of each group, from
+ * their last ones back, half of the threads on each chunk: the rows that
+ * k_gn_stats read last are still in this XCD's L2. us of both kernels at 82944
+ * rows of 256 floats and 4 x 20736 of 256 bf16: 42.3 and 27.0; from the first
+ * rows on 44.8 and 28.7. */
 template <int DT, int V>
 __global__ __launch_bounds__(TH) void k_gn_apply(const struct groupnorm_desc d)
 {
@@ -415,14 +425,20 @@ __global__ __launch_bounds__(TH) void k_gn_apply(const struct groupnorm_desc d)
     const int cv = d.C / V, gv = d.C / d.groups / V;
     long r0, r1;
 
-    chunk_rows(d, &r0, &r1);
-    const int w = min(cv, TH), lanes = TH / w;
-    const int col = t % w, row = t / w;
+    const int w = min(cv, TH), all = TH / w;
+    const int two = all % 2 == 0, lanes = two ? all / 2 : all;
+    const int col = t % w, row = two ? t / w >> 1 : t / w;
+
+    if (two)
+        chunk_rows(d, d.chunks, 2 * blockIdx.x + (t / w & 1), &r0, &r1);
+    else
+        chunk_rows(d, d.chunks / 2, blockIdx.x, &r0, &r1);
     const long n = row < lanes ? (r1 - r0 - row + lanes - 1) / lanes : 0;
+    const long last = r0 + row + (n - 1) * lanes;
     stream<DT, V, AHEAD_APPLY> in;
 
     /* The first rows, on their way during the sums. */
-    in.start(d.X, d.xo + b * d.xs0 + (r0 + row) * d.xld + (long)col * V, (long)lanes * d.xld, n);
+    in.start(d.X, d.xo + b * d.xs0 + last * d.xld + (long)col * V, -(long)lanes * d.xld, n);
     if (d.stats)
         for (int g = t; g < d.groups; g += TH)
             st[g] = ((const struct stat *)d.stats)[b * d.groups + g];
@@ -436,8 +452,7 @@ __global__ __launch_bounds__(TH) void k_gn_apply(const struct groupnorm_desc d)
     __syncthreads();
     for (int c = col; c < cv && n > 0; c += w) {
         if (c != col)
-            in.start(d.X, d.xo + b * d.xs0 + (r0 + row) * d.xld + (long)c * V,
-                     (long)lanes * d.xld, n);
+            in.start(d.X, d.xo + b * d.xs0 + last * d.xld + (long)c * V, -(long)lanes * d.xld, n);
         const struct stat q = st[c / gv];
         float a[V], be[V];
 
@@ -447,9 +462,9 @@ __global__ __launch_bounds__(TH) void k_gn_apply(const struct groupnorm_desc d)
             be[e] = d.b ? d.b[c * V + e] : 0.0f;
         }
         with_act(d.act, [&](auto act) {
-            char *y = (char *)d.Y + vec<DT, V>::size *
-                                        (d.yo + b * d.ys0 + (r0 + row) * d.yld + (long)c * V);
-            const long ystep = (long)lanes * d.yld;
+            char *y = (char *)d.Y +
+                      vec<DT, V>::size * (d.yo + b * d.ys0 + last * d.yld + (long)c * V);
+            const long ystep = -(long)lanes * d.yld;
 
             in.run([&](vec<DT, V> &x, long k) {
 #pragma unroll
@@ -472,12 +487,22 @@ static void plan(struct groupnorm_desc *d)
     long chunks = 1;
 
     if (elems > (d->C / d->groups * (d->dt == DT_F32 ? 4 : 2) < 16 ? SPLIT_ABOVE_NARROW : SPLIT_ABOVE)) {
-        chunks = (2L * cu + d->nb - 1) / d->nb;
+        /* Two workgroups per compute unit, none left over: 3, 7, 40 batches of
+         * 20736 rows of 256 bf16 22.5, 38.5, 250 us; with those that ceil(512 /
+         * batches) has 34, 59, 317. Beyond as many batches as compute units
+         * several rounds even out: 300 of 5184 rows 493, with two chunks 564. */
+        chunks = 2L * cu / d->nb;
+        if (chunks < 2)
+            chunks = 16L * cu / d->nb;
         /* Two vectors of eight per thread. */
         if (chunks > d->rows * d->C / (16 * TH))
             chunks = d->rows * d->C / (16 * TH);
         if (chunks > d->rows)
             chunks = d->rows;
+        /* Pairs; and XCDs that match (see k_gn_stats) where that idles at most
+         * a fifth: 17 batches 84.7 and, in 16 chunks for 30, 100.7; 7 batches
+         * 42.3 in 72 chunks, 38.5 in 64. */
+        chunks &= chunks >= 64 ? ~15L : ~1L;
         if (chunks < 2)
             chunks = 2;
     }
@@ -514,7 +539,7 @@ template <int DT, int V> static int run(const struct groupnorm_desc *d, hipStrea
         }
         if (err != hipSuccess)
             return err;
-        hipLaunchKernelGGL((k_gn_apply<DT, V>), dim3((d->chunks + 1) / 2, d->nb), dim3(TH),
+        hipLaunchKernelGGL((k_gn_apply<DT, V>), dim3(d->chunks / 2, d->nb), dim3(TH),
                            d->groups * sizeof(struct stat), s, *d);
     }
     return hipGetLastError();
@@ -538,8 +563,9 @@ extern "C" int launch_groupnorm(struct groupnorm_desc *d, void *ws, size_t ws_by
         d->chunks = 1;
     d->part = (float *)ws;
     /* A launch of its own for the sums where every workgroup would read more
-     * than 128 KiB of them. */
-    d->stats = d->chunks > 1 && (long)d->chunks * d->groups > 8192
+     * than 64 KiB of them: 3 batches of 5184 rows of 256 halves, 32 groups 17.7
+     * us and 19.7, 82944 rows of 256 floats, 8 groups 41.3 and 40.0. */
+    d->stats = d->chunks > 1 && (long)d->chunks * d->groups > 4096
                    ? (char *)ws + 16 * (size_t)d->nb * d->groups * d->chunks
                    : NULL;
     return d->dt == DT_F32   ? run_dt<DT_F32>(d, (hipStream_t)stream)

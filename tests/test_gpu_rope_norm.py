@@ -496,3 +496,13 @@ def test_slices_of_one_matrix(hip, env, t, D):
         calls(lambda q, k, v, o: hip.rope_rows(m, nb, H, n, D, D, layout, q, o, tab, n))
     calls(lambda q, k, v, o: hip.groupnorm(m, nb, n, W, 4, q, o))
     be.release(tab)
+
+
+@pytest.mark.parametrize("nb,rows,C,G", [(3, 3000, 64, 8), (7, 1500, 96, 8), (1, 9000, 64, 2),
+                                         (300, 129, 256, 1), (1, 2, 20000, 1), (1, 40000, 3, 1),
+                                         (2, 1000, 1048, 4), (5, 2700, 256, 64)])
+def test_norm_rounds(hip, env, nb, rows, C, G):
+    """Chunks of rows in whole pairs and rounds, with and without XCDs that
+    match, rows fewer than chunks, rows of more columns than threads."""
+    check_norm(hip, env, C, sc.F16, nb, rows, C, G)
+    check_norm(hip, env, G, sc.F32, nb, rows, C, G, lay="odd")
