@@ -27,11 +27,12 @@
  */
 #include "k_xattn.h"
 
-/* DP: head width padded to 32, 64, 128 or 256. WM waves share the rows of a
+/* DP: head width padded to 32, 64, 128 or 256, of which the first DB blocks of 32
+ * hold columns. WM waves share the rows of a
  * workgroup, the rest of its four the keys of a tile; WM = 8 is eight waves, each
  * with rows of its own. TK: keys of a tile. ST: tiles in LDS, ST - 1 of them
  * ahead. VEC: the rows of all operands are whole 16-byte pieces. */
-template <int DT, int DP, int WM, int TK, int ST, int OCC, bool VEC>
+template <int DT, int DP, int DB, int WM, int TK, int ST, int OCC, bool VEC>
 __global__ __launch_bounds__(WM == 8 ? 512 : 256, OCC) void k_xattn(const struct xattn_desc a)
 {
     constexpr int S = xt<DT>::size;
@@ -41,6 +42,7 @@ __global__ __launch_bounds__(WM == 8 ? 512 : 256, OCC) void k_xattn(const struct
     constexpr int NB = KW / 32;          /* 32-key blocks of them */
     constexpr int RB = DP * S;           /* bytes of a row */
     constexpr int CH = RB / 16;          /* 16-byte chunks of a row */
+    constexpr int QS = DB * S;           /* steps of 32 bytes of the first product */
     constexpr int NI = TK * RB / (1024 * NW); /* copies of a wave for K or V: 1 KiB each */
     constexpr int MERGE = WK > 1 ? 4 * 32 * (DP + 4) * 4 + 4 * 32 * 8 : 0;
     typedef row_k<RB> rk;
@@ -89,10 +91,11 @@ __global__ __launch_bounds__(WM == 8 ? 512 : 256, OCC) void k_xattn(const struct
 
     /* Copy i of this wave fills rows (w NI + i) RPK on of a tile; lane l's 16
      * bytes are of row l / CH of them. koff, voff: their offsets in memory from
-     * the copy's first row. lk, lv: where the wave's copies go in slot 0. */
+     * the copy's first row (columns of blocks that are not used stand for any:
+     * the first ones). lk, lv: where the wave's copies go in slot 0. */
     const int lrow = l / CH;
     const int ck = 16 * ((l % CH) ^ rk::swz(lrow)), cv = 16 * ((l % CH) ^ rv::swz(lrow));
-    const uint32_t koff = lrow * kstep + ck, voff = lrow * vstep + cv;
+    const uint32_t koff = lrow * kstep + (ck < hdb ? ck : 0), voff = lrow * vstep + (cv < hdb ? cv : 0);
     const unsigned lk = (unsigned)(uintptr_t)lds + w * NI * (1024 + rk::PAD);
     const unsigned lv = (unsigned)(uintptr_t)lds + KT + w * NI * (1024 + rv::PAD);
     /* Starts the copies of a tile of which every row is whole, from rows kt and
@@ -112,7 +115,7 @@ __global__ __launch_bounds__(WM == 8 ? 512 : 256, OCC) void k_xattn(const struct
     auto copy = [&](int j0, int st) {
         const int last = je - 1 - j0, w0 = w * NI * rk::RPK;
 
-        if (VEC && a.hd == DP && last >= TK - 1) {
+        if (VEC && a.hd == 32 * DB && last >= TK - 1) {
             copy_full(kb + (long)(j0 + w0) * kstep, vb + (long)(j0 + w0) * vstep, st);
             return;
         }
@@ -149,26 +152,26 @@ __global__ __launch_bounds__(WM == 8 ? 512 : 256, OCC) void k_xattn(const struct
     const int r = r0 + wm * 32 + lr;
     const int rc = min(r, rows - 1);
     const int hq = a.grp == 1 ? 0 : rc / nq, iq = rc - hq * nq;
-    u32x4 qf[CH / 2];
+    u32x4 qf[QS];
     {
         const char *q = (const char *)a.Q +
                         S * (a.qo + (long)b * a.qs0 + (long)(kh * a.grp + hq) * a.qs1 +
                              (long)iq * a.qld);
 
 #pragma unroll
-        for (int i = 0; i < CH / 2; i++)
+        for (int i = 0; i < QS; i++)
             qf[i] = row16<DT, VEC>(q, 16 * (2 * i + h), hdb);
     }
     /* Q has arrived: left to its first use, the wait for it would stand inside
      * the loop and wait for the copies of the next tile there each time. */
 #pragma unroll
-    for (int i = 0; i < CH / 2; i++)
+    for (int i = 0; i < QS; i++)
         asm volatile("" : "+v"(qf[i]));
-    f32x16 o[DP / 32];
+    f32x16 o[DB];
     float m = NEG_INF, sum = 0.0f;
 
 #pragma unroll
-    for (int i = 0; i < DP / 32; i++)
+    for (int i = 0; i < DB; i++)
         o[i] = f32x16{0};
     /* This wave's keys of the tile in slot st: all of them, or those whose
      * bit in keep is set. */
@@ -185,13 +188,13 @@ __global__ __launch_bounds__(WM == 8 ? 512 : 256, OCC) void k_xattn(const struct
             s[n] = f32x16{0};
         if (half) {
 #pragma unroll
-            for (int i = 0; i < CH / 2; i++)
+            for (int i = 0; i < QS; i++)
                 s[0] = k_step<DT>(*(const u32x4 *)(ldk + rk::at(lr) + 16 * ((2 * i + h) ^ rk::swz(lr))),
                                   qf[i], s[0]);
         }
         else {
 #pragma unroll
-            for (int i = 0; i < CH / 2; i++)
+            for (int i = 0; i < QS; i++)
 #pragma unroll
                 for (int n = 0; n < NB; n++)
                     s[n] = k_step<DT>(*(const u32x4 *)(ldk + rk::at(n * 32) + rk::at(lr) +
@@ -231,7 +234,7 @@ __global__ __launch_bounds__(WM == 8 ? 512 : 256, OCC) void k_xattn(const struct
             m = mn;
             sum *= f;
 #pragma unroll
-            for (int d = 0; d < DP / 32; d++)
+            for (int d = 0; d < DB; d++)
 #pragma unroll
                 for (int i = 0; i < 16; i++)
                     o[d][i] *= f;
@@ -260,7 +263,7 @@ __global__ __launch_bounds__(WM == 8 ? 512 : 256, OCC) void k_xattn(const struct
                         ldv + rv::at(n * 32 + 8 * (i / 4)) + rv::at(i % 4 + 4 * h) + 4 * lr;
 
 #pragma unroll
-                    for (int d = 0; d < DP / 32; d++)
+                    for (int d = 0; d < DB; d++)
                         o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(
                             *(const float *)(vr + 128 * d), s[n][i], o[d], 0, 0, 0);
                 }
@@ -277,7 +280,7 @@ __global__ __launch_bounds__(WM == 8 ? 512 : 256, OCC) void k_xattn(const struct
                     for (int i = 0; i < 4; i++)
                         p[i] = pack2<DT>(s[n][8 * hf + 2 * i], s[n][8 * hf + 2 * i + 1]);
 #pragma unroll
-                    for (int d = 0; d < DP / 32; d++) {
+                    for (int d = 0; d < DB; d++) {
                         const char *vd = vr + 16 * ((4 * d + c0) ^ rv::swz(row));
                         const u32x2 v0 = lds_tr(vd), v1 = lds_tr(vd + rv::at(8));
                         const u32x4 vf = {v0.x, v0.y, v1.x, v1.y};
@@ -291,7 +294,7 @@ __global__ __launch_bounds__(WM == 8 ? 512 : 256, OCC) void k_xattn(const struct
     int j0 = jb, st = 0;
 
     /* Whole tiles whose copies ahead are whole tiles too: nothing to check. */
-    if (VEC && a.hd == DP && !mk) {
+    if (VEC && a.hd == 32 * DB && !mk) {
         const long ahead = j0 + (ST - 1) * TK + w * NI * rk::RPK;
         const char *kt = kb + ahead * kstep, *vt = vb + ahead * vstep;
 
@@ -352,7 +355,7 @@ __global__ __launch_bounds__(WM == 8 ? 512 : 256, OCC) void k_xattn(const struct
         const float f = __builtin_amdgcn_exp2f(m - ref);
 
 #pragma unroll
-        for (int d = 0; d < DP / 32; d++)
+        for (int d = 0; d < DB; d++)
 #pragma unroll
             for (int q = 0; q < 4; q++) {
                 f32x4 t;
@@ -366,7 +369,7 @@ __global__ __launch_bounds__(WM == 8 ? 512 : 256, OCC) void k_xattn(const struct
         /* Wave w adds and keeps the d blocks wk, wk + WK, ... of its rows:
          * the registers it stores below. */
 #pragma unroll
-        for (int d = 0; d < DP / 32; d++)
+        for (int d = 0; d < DB; d++)
             if (d % WK == wk)
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
@@ -394,7 +397,7 @@ __global__ __launch_bounds__(WM == 8 ? 512 : 256, OCC) void k_xattn(const struct
             ((float2 *)(a.part + a.part_ml))[ur] = float2{m, sum};
         if (jb < je) {
 #pragma unroll
-            for (int d = 0; d < DP / 32; d++)
+            for (int d = 0; d < DB; d++)
                 if (d % WK == wk)
 #pragma unroll
                     for (int q = 0; q < 4; q++) {
@@ -419,7 +422,7 @@ __global__ __launch_bounds__(WM == 8 ? 512 : 256, OCC) void k_xattn(const struct
                                         (long)iq * a.old);
 
 #pragma unroll
-    for (int d = 0; d < DP / 32; d++)
+    for (int d = 0; d < DB; d++)
         if (d % WK == wk)
             put_block<DT, VEC>(op, 32 * d, a.hd, h, o[d], inv);
 }
@@ -833,15 +836,28 @@ extern "C" size_t xattn_ws(struct xattn_desc *d)
     return 4 * part_ml(d) + 8 * (size_t)d->splits * d->units * d->grp * d->Nq;
 }
 
-template <int DT, int DP, int WM, int TK, int ST, int OCC, bool VEC = true>
-static int run(const struct xattn_desc *d, hipStream_t s)
+template <int DT, int DP, int WM, int TK, int ST, int OCC, bool VEC = true, int DB = DP / 32>
+static int run_blocks(const struct xattn_desc *d, hipStream_t s)
 {
     const unsigned grid = d->heads_first ? item_grid(d->tiles, d->units)
                                          : item_grid(d->units * d->splits, d->tiles);
 
-    hipLaunchKernelGGL((k_xattn<DT, DP, WM, TK, ST, OCC, VEC>), dim3(grid),
+    hipLaunchKernelGGL((k_xattn<DT, DP, DB, WM, TK, ST, OCC, VEC>), dim3(grid),
                        dim3(WM == 8 ? 512 : 256), 0, s, *d);
     return hipGetLastError();
+}
+
+/* Heads of up to three quarters of the padded width take a kernel without the
+ * last quarter's products. us, against the products of zeros: 8 heads of 96
+ * bf16, 5184 x 5184 108 and 146; 2 of 192, 3000 x 3000 39 and 63; 32 of 80,
+ * 1024 x 1024 24.6 and 27.0; 12 of 96 floats, 449 x 2533 97 and 126. */
+template <int DT, int DP, int WM, int TK, int ST, int OCC, bool VEC = true>
+static int run(const struct xattn_desc *d, hipStream_t s)
+{
+    if constexpr (VEC && DP >= 128)
+        if (d->hd <= DP / 4 * 3)
+            return run_blocks<DT, DP, WM, TK, ST, OCC, VEC, DP / 128 * 3>(d, s);
+    return run_blocks<DT, DP, WM, TK, ST, OCC, VEC>(d, s);
 }
 
 template <int DT, int DP, int NB> static int run_few(const struct xattn_desc *d, hipStream_t s)

@@ -234,3 +234,30 @@ def test_many_rows_wide_heads(hip, env, t, D, H, KV, nq, nk):
     check(hip, env, D + 1, sc.TYPES[t], nb, H, KV, D, nq, nk, kmask=mask, klen=[nk - 33] * nb,
           qlen=[nq - 300] * nb)
     check(hip, env, D + 2, sc.TYPES[t], nb, H, KV, D, nq, nk, klen=[65] * nb)
+
+
+@pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("D", [65, 72, 80, 96, 104, 160, 192, 200])
+def test_three_quarters_of_a_width(hip, env, t, D):
+    """Heads whose last quarter of columns is empty, and just not: whole tiles
+    and others, few rows and many, splits; infinities in what is masked."""
+    dt = sc.TYPES[t]
+    for nq, nk, kw in ((40, 300, {}), (130, 640, {}), (1, 1500, {}), (300, 1030, {})):
+        check(hip, env, D + nq, dt, 2, 2, 1, D, nq, nk, **kw)
+    check(hip, env, D, dt, 2, 2, 2, D, 70, 400, klen=[399, 1], bad=np.inf)
+    mask = (np.random.default_rng(D).random((2, 400)) < 0.3).astype(np.uint8)
+    check(hip, env, D, dt, 2, 2, 2, D, 70, 400, kmask=mask, lay="wide")
+
+
+def test_columns_of_neighbours_are_not_read(hip, env):
+    """Heads of 96 side by side: a head of infinities leaves the next alone."""
+    def change(q, k, v):
+        k[:, :, 1], v[:, :, 1] = np.inf, np.nan
+
+    for dt in (sc.F16, sc.F32):
+        got, q, k, v, keep, scale = run(hip, env, 5, dt, 1, 3, 3, 96, 64, 512, change=change)
+        for h in (0, 2):
+            o, av, top, prod = sc.cross(q[:, :, h:h + 1], k[:, :, h:h + 1], v[:, :, h:h + 1], keep,
+                                        scale)
+            lim = sc.cross_bound(o, av, top, prod, 96, 512, dt, v[:, :, h:h + 1])
+            assert (np.abs(got[:, :, h:h + 1] - o) <= lim).all()
