@@ -509,12 +509,17 @@ static void plan(struct groupnorm_desc *d)
     d->chunks = (int)chunks;
 }
 
-extern "C" size_t groupnorm_ws_bytes(struct groupnorm_desc *d)
+static size_t part_bytes(const struct groupnorm_desc *d)
 {
-    plan(d);
     return d->chunks > 1
                ? (size_t)d->nb * d->groups * (16 * (size_t)d->chunks + sizeof(struct stat))
                : 0;
+}
+
+extern "C" size_t groupnorm_ws_bytes(struct groupnorm_desc *d)
+{
+    plan(d);
+    return part_bytes(d);
 }
 
 template <int DT, int V> static int run(const struct groupnorm_desc *d, hipStream_t s)
@@ -557,9 +562,7 @@ template <int DT> static int run_dt(const struct groupnorm_desc *d, hipStream_t 
 
 extern "C" int launch_groupnorm(struct groupnorm_desc *d, void *ws, size_t ws_bytes, void *stream)
 {
-    const size_t need = groupnorm_ws_bytes(d);
-
-    if (need && (!ws || ws_bytes < need))
+    if (!ws || ws_bytes < part_bytes(d))
         d->chunks = 1;
     d->part = (float *)ws;
     /* A launch of its own for the sums where every workgroup would read more

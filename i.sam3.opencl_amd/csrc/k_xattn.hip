@@ -80,8 +80,9 @@ __global__ __launch_bounds__(WM == 8 ? 512 : 256, OCC) void k_xattn(const struct
 
     if (r0 >= rows)
         return;
-    const int per_split = ((nk + a.splits - 1) / a.splits + TK - 1) / TK * TK;
-    const int jb = min(nk, split * per_split), je = min(nk, jb + per_split);
+    /* Every splits-th tile, so that splits have like shares of what a mask
+     * leaves. */
+    const int hop = TK * a.splits, jb = TK * split, je = nk;
     const int hdb = a.hd * S;
 
     const char *const kb = (const char *)a.K + S * (a.ko + (long)b * a.ks0 + (long)kh * a.ks1);
@@ -146,8 +147,8 @@ __global__ __launch_bounds__(WM == 8 ? 512 : 256, OCC) void k_xattn(const struct
     /* The first tiles, on their way while Q is read. */
 #pragma unroll
     for (int i = 0; i < ST - 1; i++)
-        if (jb + i * TK < je)
-            copy(jb + i * TK, i);
+        if (jb + i * hop < je)
+            copy(jb + i * hop, i);
     /* This lane's row: query and head, and its part of Q. */
     const int r = r0 + wm * 32 + lr;
     const int rc = min(r, rows - 1);
@@ -295,29 +296,29 @@ __global__ __launch_bounds__(WM == 8 ? 512 : 256, OCC) void k_xattn(const struct
 
     /* Whole tiles whose copies ahead are whole tiles too: nothing to check. */
     if (VEC && a.hd == 32 * DB && !mk) {
-        const long ahead = j0 + (ST - 1) * TK + w * NI * rk::RPK;
+        const long ahead = j0 + (ST - 1) * hop + w * NI * rk::RPK;
         const char *kt = kb + ahead * kstep, *vt = vb + ahead * vstep;
 
-        for (; j0 + ST * TK <= je; j0 += TK) {
+        for (; j0 + (ST - 1) * hop + TK <= je; j0 += hop) {
             copies_and_barrier<(ST - 2) * 2 * NI>();
             copy_full(kt, vt, st == 0 ? ST - 1 : st - 1);
-            kt += (long)TK * kstep;
-            vt += (long)TK * vstep;
+            kt += (long)hop * kstep;
+            vt += (long)hop * vstep;
             attend_tile(yes{}, st, 0);
             st = st + 1 == ST ? 0 : st + 1;
         }
     }
-    for (; j0 < je; j0 += TK, st = st + 1 == ST ? 0 : st + 1) {
+    for (; j0 < je; j0 += hop, st = st + 1 == ST ? 0 : st + 1) {
         const int j = min(j0 + wk * KW + (l & (KW - 1)), je - 1);
         const bool drop = mk && mk[j] == 0;
 
         /* This tile has landed, and the slot of the one before is free. */
-        if (ST > 2 && j0 + (ST - 2) * TK < je)
+        if (ST > 2 && j0 + (ST - 2) * hop < je)
             copies_and_barrier<(ST - 2) * 2 * NI>();
         else
             copies_and_barrier<0>();
-        if (j0 + (ST - 1) * TK < je)
-            copy(j0 + (ST - 1) * TK, st == 0 ? ST - 1 : st - 1);
+        if (j0 + (ST - 1) * hop < je)
+            copy(j0 + (ST - 1) * hop, st == 0 ? ST - 1 : st - 1);
         /* Which of this wave's keys count. */
         const uint64_t keep = __ballot(l < KW && j0 + wk * KW + l < je && !drop);
 
@@ -730,6 +731,19 @@ static int padded(int hd)
     return hd <= 32 ? 32 : hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
 }
 
+/* Time of floats in f32 plans, in 32 rows x one key on a SIMD, wm waves' rows in
+ * s splits: the compute unit with most workgroups, their start (and, with the
+ * keys in four waves, the copies, which bind: 1.2), the merge's launch and the
+ * splits' records. */
+static double cost_f32(const struct xattn_desc *d, int wm, int s, long rows, long cu)
+{
+    const long wg = d->units * ((rows + 32 * wm - 1) / (32 * wm)) * s;
+    const double keys = ((d->Nk + s - 1) / s + 63) / 64 * 64.0, rounds = (wg + cu - 1) / cu;
+    const double c = rounds * (wm == 1 ? 1.2 * (keys + 128) : wm * (keys + 64));
+
+    return s == 1 ? c : c + 12000.0 / padded(d->hd) + 0.005 * d->units * rows * s;
+}
+
 /* How the work is cut. A workgroup of wm x 32 rows walks all keys of its rows,
  * or one of several splits of them whose sums a second launch adds up. More rows
  * share each copied tile; fewer make more workgroups, whose waves then share
@@ -772,7 +786,7 @@ static void plan(struct xattn_desc *d)
     }
     if (!d->vec)
         wm = rb >= 1024 ? 4 : 2;
-    else if (d->dt != DT_F32 && rb >= 256 && rows >= (rb == 256 ? 1024 : 256) && d->Nk > 256) {
+    if (d->vec && d->dt != DT_F32 && rb >= 256 && rows >= (rb == 256 ? 1024 : 256) && d->Nk > 256) {
         /* The copies into LDS are what such heads wait for (6 to 8 TB/s): 256 rows
          * share them, one workgroup of eight waves per compute unit and as many
          * splits as make one for each, unless they get short. us, against the
@@ -797,13 +811,34 @@ static void plan(struct xattn_desc *d)
             return;
         }
     }
-    if (d->vec && d->Nk > 256) {
+    if (d->vec && d->dt == DT_F32 && rows > 64) {
+        /* Float products fill the SIMDs, so that even loads of the compute units
+         * count most: the cheapest cut. us, against the rules below: 449 x 2533,
+         * 12 heads of 96 77 and 101; 1000 x 1000, 8 heads of 64 26 and 41, of
+         * 128 50 and 77; 5184 x 5184, 8 heads of 128 857 and 1079. */
+        static const int cuts[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+        double best = 0.0;
+
+        for (int w = 4; w >= (rb >= 1024 ? 4 : rb >= 512 ? 2 : 1); w /= 2)
+            for (int n : cuts) {
+                const double c = cost_f32(d, w, n, rows, cu);
+
+                if (n > 1 && (d->Nk <= 256 || d->Nk / n < 192))
+                    break;
+                if (best == 0.0 || c < best) {
+                    best = c;
+                    wm = w;
+                    d->splits = n;
+                }
+            }
+    }
+    else if (d->Nk > 256) {
         const int most_rows = wm;
         long want = 2 * cu;
 
-        if (wm == 4 && least <= 2 && WG(4) < 2 * cu)
+        if (d->vec && wm == 4 && least <= 2 && WG(4) < 2 * cu)
             wm = 2;
-        if (wm == 2 && least == 1 && WG(2) < cu + cu / 4)
+        if (d->vec && wm == 2 && least == 1 && WG(2) < cu + cu / 4)
             wm = 1;
         if (rows <= 64 ? WG(wm) < 2 * cu : WG(wm) < cu / 2) {
             wm = most_rows;
@@ -828,12 +863,17 @@ static size_t part_ml(const struct xattn_desc *d)
     return ((size_t)d->splits * d->units * d->grp * d->Nq * d->hd + 3) & ~(size_t)3;
 }
 
+static size_t part_bytes(const struct xattn_desc *d)
+{
+    return d->splits == 1
+               ? 0
+               : 4 * part_ml(d) + 8 * (size_t)d->splits * d->units * d->grp * d->Nq;
+}
+
 extern "C" size_t xattn_ws(struct xattn_desc *d)
 {
     plan(d);
-    if (d->splits == 1)
-        return 0;
-    return 4 * part_ml(d) + 8 * (size_t)d->splits * d->units * d->grp * d->Nq;
+    return part_bytes(d);
 }
 
 template <int DT, int DP, int WM, int TK, int ST, int OCC, bool VEC = true, int DB = DP / 32>
@@ -905,7 +945,7 @@ template <int DT, int DP> static int run_wm(const struct xattn_desc *d, hipStrea
     }
     if constexpr (RB <= 128)
         return run<DT, DP, 1, 128, 2, 2>(d, s);
-    else if constexpr (RB == 256)
+    else if constexpr (RB == 256 && DT == DT_F32)
         return run<DT, DP, 1, 128, 2, 1>(d, s);
     return hipErrorInvalidValue;
 }
@@ -939,12 +979,9 @@ template <int DT> static int run_dt(struct xattn_desc *d, hipStream_t s)
 
 extern "C" int launch_xattn(struct xattn_desc *d, void *ws, size_t ws_bytes, void *stream)
 {
-    const size_t need = xattn_ws(d);
-
-    if (need && (!ws || ws_bytes < need)) {
-        /* One workgroup per row tile walks all keys. */
+    /* Without the room one workgroup per row tile walks all keys. */
+    if (!ws || ws_bytes < part_bytes(d))
         d->splits = 1;
-    }
     d->part = (float *)ws;
     d->part_ml = d->splits > 1 ? (long)part_ml(d) : 0;
     if (d->dt == DT_F32)

@@ -363,8 +363,9 @@ struct xattn_desc {
     long part_ml;
 };
 
-/* Bytes of workspace that lets launch_xattn split the keys (0: it does not
- * want to); with less, or NULL, one workgroup walks all keys of its rows. */
+/* Plans the launch of d; bytes of workspace that lets it split the keys (0: it
+ * does not want to). With less, or NULL, one workgroup walks all keys of its
+ * rows. Called before launch_xattn. */
 size_t xattn_ws(struct xattn_desc *d);
 int launch_xattn(struct xattn_desc *d, void *ws, size_t ws_bytes, void *stream);
 
@@ -414,8 +415,9 @@ struct groupnorm_desc {
     void *stats;
 };
 
-/* Workspace (0: none wanted); with less, or NULL, one workgroup per (batch,
- * group) walks all rows. */
+/* Plans the launch of d; workspace (0: none wanted). With less, or NULL, one
+ * workgroup per (batch, group) walks all rows. Called before
+ * launch_groupnorm. */
 size_t groupnorm_ws_bytes(struct groupnorm_desc *d);
 int launch_groupnorm(struct groupnorm_desc *d, void *ws, size_t ws_bytes, void *stream);
 

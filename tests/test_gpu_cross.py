@@ -261,3 +261,26 @@ def test_columns_of_neighbours_are_not_read(hip, env):
                                         scale)
             lim = sc.cross_bound(o, av, top, prod, 96, 512, dt, v[:, :, h:h + 1])
             assert (np.abs(got[:, :, h:h + 1] - o) <= lim).all()
+
+
+@pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("H,KV,D,nq,nk", [(2, 2, 20, 1, 3001), (4, 2, 130, 3, 1200), (1, 1, 7, 200, 2050),
+                                          (3, 1, 64, 40, 900)])
+@pytest.mark.parametrize("ws", [False, True])
+def test_splits_of_odd_layouts(hip, env, t, H, KV, D, nq, nk, ws):
+    """Rows that do not start on 16 bytes, few of them over many keys."""
+    be, m = env
+    dt = sc.TYPES[t]
+    assert hip.cross_attend_ws(m, 2, H, KV, D, nq, nk, dt) > 0
+    check(hip, env, D, dt, 2, H, KV, D, nq, nk, lay="odd", ws=ws)
+    check(hip, env, D, dt, 2, H, KV, D, nq, nk, lay="odd", klen=[nk - 1, 3], qlen=[nq, 1], ws=ws)
+
+
+@pytest.mark.parametrize("H,KV,D,nq,nk", [(12, 12, 96, 449, 2533), (8, 8, 64, 500, 500),
+                                          (4, 2, 32, 230, 3100), (1, 1, 256, 700, 2001),
+                                          (16, 16, 128, 300, 230), (2, 2, 64, 65, 1000)])
+def test_cuts_of_floats(hip, env, H, KV, D, nq, nk):
+    check(hip, env, D, sc.F32, 1, H, KV, D, nq, nk)
+    check(hip, env, D, sc.F32, 1, H, KV, D, nq, nk, klen=[nk // 3], lay="wide")
+    mask = (np.random.default_rng(D).random((1, nk)) < 0.5).astype(np.uint8)
+    check(hip, env, D, sc.F32, 1, H, KV, D, nq, nk, kmask=mask, qlen=[nq - 7], lay="heads")
