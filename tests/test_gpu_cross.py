@@ -284,3 +284,24 @@ def test_cuts_of_floats(hip, env, H, KV, D, nq, nk):
     check(hip, env, D, sc.F32, 1, H, KV, D, nq, nk, klen=[nk // 3], lay="wide")
     mask = (np.random.default_rng(D).random((1, nk)) < 0.5).astype(np.uint8)
     check(hip, env, D, sc.F32, 1, H, KV, D, nq, nk, kmask=mask, qlen=[nq - 7], lay="heads")
+
+
+@pytest.mark.parametrize("t", ALL)
+@pytest.mark.parametrize("D,nq", [(32, 5), (64, 300), (96, 70), (128, 1), (128, 600), (256, 40), (256, 300),
+                                  (20, 33)])
+def test_long_masks(hip, env, t, D, nq):
+    """Masks over more than 512 keys: empty tiles at the start, in the middle,
+    at the end, more than 64 tiles of them, one key in all, none; bytes other
+    than one; keys that end before the mask does, within its first four bytes
+    too."""
+    nb, nk = 8, 9001 if D < 128 else 2601
+    g = np.random.default_rng(D + nq)
+    mask = np.zeros((nb, nk), np.uint8)
+    mask[0, :7], mask[0, -nk // 8:] = 255, 128
+    mask[1, nk // 2:nk // 2 + 100] = g.integers(0, 3, 100)
+    mask[2, -1] = 1
+    mask[3, 0] = 16
+    mask[5] = g.random(nk) < 0.02
+    mask[6], mask[7] = 1, 1
+    klen = [nk, nk, nk, nk, nk, nk - 1, 3, 700]
+    check(hip, env, D, sc.TYPES[t], nb, 2, 1, D, nq, nk, kmask=mask, klen=klen)
