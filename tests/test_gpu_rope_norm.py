@@ -372,7 +372,9 @@ def test_run_of_operators(hip, env, t):
 
 def capture(hip, be, call):
     """The call captured on the backend's stream: a replay function."""
-    rt = ctypes.CDLL("libamdhip64.so")
+    # The runtime that the library is linked to: a process that imports torch
+    # after it holds another one too, whose streams these are not.
+    rt = hip.lib()
     s = ctypes.c_void_p(be._b.stream)
     graph, ex = ctypes.c_void_p(), ctypes.c_void_p()
     assert rt.hipStreamBeginCapture(s, 2) == 0
