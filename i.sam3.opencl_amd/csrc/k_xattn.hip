@@ -836,10 +836,13 @@ static double cost_f32(const struct xattn_desc *d, int wm, int s, long rows, lon
  * So: as many rows as still give two workgroups per compute unit, or one and a
  * quarter with wm 2; splits only where even the least rows leave half of the
  * compute units idle, and then two workgroups for each.
- * With few rows the splits' sums are small, and lengths may differ: 16
- * sequences of 40 to 100 % of 8192 keys, 8 key heads of 128: 79 us with eight
- * splits, 89 with four, 83 with sixteen (four workgroups per compute unit);
- * but 64 sequences of 2048 67 without and 75 with two. */
+ * With up to 64 rows (tokens being made) one workgroup per compute unit is
+ * enough, if that makes eight splits: one token over 8192 keys, 16 / 48 key heads
+ * of 128 / 64 18.5 / 21.7, with four workgroups per compute unit 21.2 / 26.0; 12 of
+ * 64 over 32768 24.3 and 31.5. Else eight, since lengths may differ: 16
+ * sequences of 40 to 100 % of 8192 keys, 8 key heads of 128 78.1, four 81.0; but
+ * 64 sequences of 2048 67 without and 75 with two. Down to 128 keys each: floats,
+ * 10 x 700, 8 heads of 64 15.3, down to 256 21.9. */
 static void plan(struct xattn_desc *d)
 {
     const long cu = dev_cu_count(), rows = (long)d->grp * d->Nq;
@@ -921,12 +924,17 @@ static void plan(struct xattn_desc *d)
         if (d->vec && wm == 2 && least == 1 && WG(2) < cu + cu / 4)
             wm = 1;
         if (rows <= 64 ? WG(wm) < 2 * cu : WG(wm) < cu / 2) {
+            const int least_keys = rows <= 64 ? 128 : 384;
+
             wm = most_rows;
-            if (rows <= 64)
-                want = 4 * cu;
+            if (rows <= 64) {
+                want = cu;
+                if (cu / WG(wm) < 8)
+                    want = 8 * WG(wm) < 4 * cu ? 8 * WG(wm) : 4 * cu;
+            }
             want /= WG(wm);
-            if (want > d->Nk / 384)
-                want = d->Nk / 384;
+            if (want > d->Nk / least_keys)
+                want = d->Nk / least_keys;
             d->splits = want < 1 ? 1 : want > 64 ? 64 : (int)want;
         }
     }
