@@ -617,7 +617,8 @@ def bmat(buf, off, ld, s0, s1):
 def borrow(ptr, nbytes, dtype=F32, what="borrowed"):
     """A handle of device memory that another allocator owns (struct hipb_buf
     is plain data): for the operators, never for hipb_release. The memory has
-    to outlive the handle's calls."""
+    to outlive the handle's calls, and what another stream writes to it to be
+    complete before them: the backend's stream waits for no other."""
     return ctypes.pointer(HipbBuf(ptr, nbytes, dtype, what.encode()))
 
 
